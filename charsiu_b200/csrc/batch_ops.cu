@@ -1,0 +1,544 @@
+// SPDX-License-Identifier: GPL-2.0-or-later
+// The operators of a batched step: argument checks, launch shapes and the C entry
+// points of include/charsiu_gpu.h. The kernels are in norm_rows.cuh, pages.cuh,
+// attn.cuh and adapters.cuh.
+//
+// Every launch has the programmatic attribute, and every kernel waits for its
+// predecessor before it reads or writes anything of the caller's.
+#include <cuda_runtime.h>
+
+#include <cstdio>
+#include <type_traits>
+
+#include "charsiu_gpu.h"
+
+#include "adapters.cuh"
+#include "attn.cuh"
+#include "layer_internal.h"
+#include "norm_rows.cuh"
+#include "pages.cuh"
+
+using namespace cgpu;
+
+namespace {
+
+constexpr uint32_t TYPE_F32 = 0, TYPE_F16 = 1, TYPE_BF16 = 30;      // GGML's numbers
+
+// The layer's GPU for the length of a call; the caller's current one after it.
+struct OnDevice {
+	int before = -1, device;
+	explicit OnDevice(const charsiu_gpu *g) : device(layer_device(g))
+	{
+		if (cudaGetDevice(&before) != cudaSuccess)
+			before = -1;
+		if (before != device)
+			cudaSetDevice(device);
+	}
+	~OnDevice()
+	{
+		if (before >= 0 && before != device)
+			cudaSetDevice(before);
+	}
+};
+
+int refuse(charsiu_gpu *g, const char *why)
+{
+	layer_whine(g, why);
+	return -1;
+}
+
+bool misaligned(const void *p, uintptr_t to)
+{
+	return (uintptr_t)p & (to - 1);
+}
+
+template <typename K, typename... Args>
+bool launch(charsiu_gpu *g, void *stream, K kernel, dim3 grid, unsigned block, size_t smem,
+	    Args... args)
+{
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = grid;
+	cfg.blockDim = dim3(block);
+	cfg.dynamicSmemBytes = smem;
+	cfg.stream = stream ? (cudaStream_t)stream : layer_stream(g);
+	cudaLaunchAttribute attr[1];
+	attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	attr[0].val.programmaticStreamSerializationAllowed = 1;
+	cfg.attrs = attr;
+	cfg.numAttrs = layer_no_pdl(g) ? 0 : 1;
+	const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+	if (e != cudaSuccess) {
+		cudaGetLastError();
+		char why[160];
+		snprintf(why, sizeof(why), "the launch failed: %s", cudaGetErrorString(e));
+		layer_whine(g, why);
+		return false;
+	}
+	layer_launched(g, 1);
+	return true;
+}
+
+// more than 48 KB of shared memory, asked for once a kernel and device
+template <typename K>
+bool allow_smem(charsiu_gpu *g, K kernel, size_t bytes, uint64_t &done)
+{
+	const uint64_t bit = 1ull << (layer_device(g) & 63);
+	if (done & bit)
+		return true;
+	if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
+	    cudaSuccess) {
+		cudaGetLastError();
+		layer_whine(g, "a kernel's shared memory was refused");
+		return false;
+	}
+	done |= bit;
+	return true;
+}
+
+// "" or why the calls would refuse this cache
+const char *pages_fault(const charsiu_gpu_pages *p)
+{
+	if (!p || !p->k || !p->v || !p->table || !p->len || !p->ref)
+		return "the cache lacks an array";
+	if (p->type != TYPE_F16 && p->type != TYPE_BF16)
+		return "the cache's type is neither fp16 nor bf16";
+	if (p->page != 16 && p->page != 32 && p->page != 64 && p->page != 128)
+		return "the cache's pages are not of 16, 32, 64 or 128 positions";
+	if (p->head_dim != 64 && p->head_dim != 128)
+		return "the cache's head_dim is neither 64 nor 128";
+	if (!p->n_layer || !p->n_pages || !p->n_head_kv || !p->n_seq || !p->max_pages)
+		return "the cache has a size of 0";
+	if (p->n_layer > 32767 || p->n_pages > (1u << 21) || p->n_head_kv > 1024 || p->n_seq > (1u << 20) ||
+	    (uint64_t)p->max_pages * p->page > 0x7fffff00ull)
+		return "the cache is larger than the calls take";
+	if (misaligned(p->k, 16) || misaligned(p->v, 16) || misaligned(p->table, 4) ||
+	    misaligned(p->len, 4) || misaligned(p->ref, 4) || misaligned(p->work, 4))
+		return "an array of the cache is misaligned";
+	if (p->layer_stride % 8 || p->page_stride % 8 || p->pos_stride % 8 || p->head_stride % 8)
+		return "a stride of the cache is not a multiple of 8";
+	if (p->pos_stride < p->head_dim || p->head_stride < p->head_dim)
+		return "the cache's positions or heads overlap";
+	return "";
+}
+
+// the start of every call on a cache: 0 to go on
+int pages_check(charsiu_gpu *g, const charsiu_gpu_pages *p, bool lists)
+{
+	if (!g || layer_dead(g))
+		return -1;
+	const char *why = pages_fault(p);
+	if (*why)
+		return refuse(g, why);
+	if (lists && !p->work)
+		return refuse(g, "the cache has no work array");
+	return 0;
+}
+
+int slots_check(charsiu_gpu *g, const charsiu_gpu_pages *p, const int32_t *slots, unsigned n)
+{
+	if (pages_check(g, p, true))
+		return -1;
+	if (n && !slots)
+		return refuse(g, "no slots");
+	if (n > PAGES_MAX_ITEMS)
+		return refuse(g, "more slots than a call takes");
+	return 0;
+}
+
+template <typename T>
+int append(charsiu_gpu *g, const charsiu_gpu_pages *p, unsigned layer, const int32_t *slots,
+	   unsigned n, unsigned t, unsigned n_head, const float *q, const float *k, const float *v,
+	   const float *rope_cs, unsigned n_ctx, void *q_out, void *stream)
+{
+	const uint64_t words = (uint64_t)n * t * (n_head + 2 * p->n_head_kv) * (p->head_dim / 8);
+	return launch(g, stream, pages_append_kernel<T>, dim3((unsigned)((words + 255) / 256)), 256, 0,
+		      *p, (uint32_t)layer, slots, words, (uint32_t)t, (uint32_t)n_head, q, k, v, rope_cs,
+		      (uint32_t)n_ctx, (T *)q_out)
+		       ? 0
+		       : -1;
+}
+
+// ---- attention ------------------------------------------------------------------
+
+const char *attention_fault(const charsiu_gpu_pages *p, const charsiu_gpu_attention *a)
+{
+	const char *why = pages_fault(p);
+	if (*why)
+		return why;
+	if (!a || !a->slots || (a->n_group && (!a->group || !a->shared)))
+		return "the batch lacks an array";
+	if (!a->n_tok || !a->n_head || a->n_head % p->n_head_kv)
+		return "n_tok is 0, or n_head no multiple of n_head_kv";
+	if ((uint64_t)a->n_seq * a->n_tok * a->n_head > 0x7fffffffull || a->n_group > a->n_seq)
+		return "the batch is larger than the call takes";
+	if (a->out_type != TYPE_F32 && a->out_type != p->type)
+		return "out_type is neither fp32 nor the cache's type";
+	return "";
+}
+
+constexpr uint32_t ATTN_CTAS_PER_SM = 3, ATTN_MAX_SPLITS = 32;
+
+// How the work is cut.
+void attention_plan(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gpu_attention *b,
+		    AttnArgs *a)
+{
+	const uint32_t gqa = b->n_head / p->n_head_kv, rows = b->n_tok * gqa;
+	const uint32_t sms = (uint32_t)layer_sms(g);
+	a->gqa = gqa;
+	a->own_tiles = (rows + ATTN_TILE_ROWS - 1) / ATTN_TILE_ROWS;
+	a->pre_units = b->n_group ? (uint32_t)(((uint64_t)b->n_seq * rows + ATTN_TILE_ROWS - 1) /
+					       ATTN_TILE_ROWS) + b->n_group
+				  : 0;
+	const uint32_t grains = (b->max_len + ATTN_GRAIN - 1) / ATTN_GRAIN + 1;
+	auto splits = [&](uint64_t ctas) {
+		uint64_t n = ctas ? ((uint64_t)ATTN_CTAS_PER_SM * sms + ctas - 1) / ctas : 1;
+		n = n > ATTN_MAX_SPLITS ? ATTN_MAX_SPLITS : n < 1 ? 1 : n;
+		return (uint32_t)(n < grains ? n : grains);
+	};
+	a->own_splits = splits((uint64_t)b->n_seq * a->own_tiles * p->n_head_kv);
+	a->pre_splits = b->n_group ? splits((uint64_t)a->pre_units * p->n_head_kv) : 0;
+}
+
+// Scratch for the pieces of this batch and of any smaller one: fewer sequences are
+// cut finer, but n sequences of c CTAs each give at most n + target / c pieces of
+// each kind, which grows with n.
+size_t attention_bytes(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gpu_attention *b)
+{
+	const uint64_t kv = p->n_head_kv, n = b->n_seq, rows = (uint64_t)b->n_tok * (b->n_head / kv);
+	const uint64_t tiles = (rows + ATTN_TILE_ROWS - 1) / ATTN_TILE_ROWS, most = ATTN_MAX_SPLITS * n;
+	const uint64_t target = ATTN_CTAS_PER_SM * (uint64_t)layer_sms(g);
+	uint64_t parts = n + target / (tiles * kv) + 1;
+	parts = parts < most ? parts : most;
+	if (b->n_group) {
+		const uint64_t pre = n + target * ATTN_TILE_ROWS / (rows * kv) + 1;
+		parts += pre < most ? pre : most;
+	}
+	return (size_t)(parts * b->n_tok * b->n_head * (p->head_dim + 1) * sizeof(float) + 15) / 16 * 16;
+}
+
+template <typename T, int HD>
+int attention(charsiu_gpu *g, const AttnArgs &a, void *stream)
+{
+	static uint64_t smem_done;
+	if (!allow_smem(g, attn_rows_kernel<T, HD>, attn_rows_smem<HD>(), smem_done))
+		return -1;
+	const uint64_t blocks = (uint64_t)a.p.n_head_kv *
+				((uint64_t)a.pre_units * a.pre_splits +
+				 (uint64_t)a.n_seq * a.own_tiles * a.own_splits);
+	if (blocks > 0x7fffffffull)
+		return refuse(g, "the batch is larger than the call takes");
+	const uint64_t rows = (uint64_t)a.n_seq * a.n_tok * a.n_head;
+	return launch(g, stream, attn_rows_kernel<T, HD>, dim3((unsigned)blocks), ATTN_WARPS * 32,
+		      attn_rows_smem<HD>(), a) &&
+			       launch(g, stream, attn_join_kernel<T, HD>,
+				      dim3((unsigned)((rows + 7) / 8)), 256, 0, a)
+		       ? 0
+		       : -1;
+}
+
+// ---- adapters --------------------------------------------------------------------
+
+const char *adapters_fault(const charsiu_gpu_adapters *s, unsigned n)
+{
+	if (!s || !n || n > (unsigned)ADAPT_MAX_SETS)
+		return "a call takes 1 to 8 adapter sets";
+	for (unsigned i = 0; i < n; i++) {
+		if (!s[i].a || !s[i].b || !s[i].rank || !s[i].scale)
+			return "an adapter set lacks an array";
+		if (s[i].type != s[0].type || (s[i].type != TYPE_F16 && s[i].type != TYPE_BF16))
+			return "the adapters' types are not all fp16 or all bf16";
+		if (!s[i].k || s[i].k % 32 || s[i].k != s[0].k || !s[i].n || s[i].n > 0x7fffff00u)
+			return "the adapters' K is not one multiple of 32, or an N is 0";
+		if (!s[i].max_rank || s[i].max_rank > 128 || (s[i].max_rank != 4 && s[i].max_rank % 8))
+			return "an adapter set's max_rank is not 4 or a multiple of 8 up to 128";
+		if (misaligned(s[i].a, 16) || misaligned(s[i].b, 16) || misaligned(s[i].rank, 4) ||
+		    misaligned(s[i].scale, 4))
+			return "an array of an adapter set is misaligned";
+		if (s[i].slots > 0x7fffffffu)
+			return "an adapter set is larger than the call takes";
+	}
+	return "";
+}
+
+// ranks a kernel holds: the largest of the sets', padded
+uint32_t adapters_ranks(const charsiu_gpu_adapters *s, unsigned n)
+{
+	uint32_t most = 0;
+	for (unsigned i = 0; i < n; i++)
+		most = s[i].max_rank > most ? s[i].max_rank : most;
+	return most <= 8 ? 8 : most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : 128;
+}
+
+// pieces of K: enough CTAs for two a multiprocessor, at least two 32-blocks a warp
+uint32_t adapters_pieces(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n, unsigned m)
+{
+	const uint64_t tiles = (uint64_t)n * ((m + ADAPT_ROWS - 1) / ADAPT_ROWS);
+	const uint32_t most = (s->k / 32 + 2 * ADAPT_WARPS - 1) / (2 * ADAPT_WARPS);
+	const uint64_t want = (2ull * layer_sms(g) + tiles - 1) / (tiles ? tiles : 1);
+	return want < 1 ? 1 : want < most ? (uint32_t)want : most;
+}
+
+// scratch for m rows, and for any fewer: pieces * m is at most the CTAs aimed at and
+// a tile's more, in rows
+size_t adapters_bytes(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n, unsigned m)
+{
+	const size_t tiles = (m + ADAPT_ROWS - 1) / ADAPT_ROWS;
+	return (2 * (size_t)layer_sms(g) + n * tiles) * ADAPT_ROWS * adapters_ranks(s, n) * sizeof(float);
+}
+
+template <typename T, int RT>
+int adapters(charsiu_gpu *g, const AdaptArgs &a, void *stream)
+{
+	const unsigned tiles = (a.m + ADAPT_ROWS - 1) / ADAPT_ROWS;
+	return launch(g, stream, adapt_shrink_kernel<T, RT>, dim3(tiles, a.pieces, a.n_sets),
+		      ADAPT_WARPS * 32, 0, a) &&
+			       launch(g, stream, adapt_expand_kernel<T, RT>, dim3(tiles, a.blocks),
+				      ADAPT_WARPS * 32, 0, a)
+		       ? 0
+		       : -1;
+}
+
+template <typename T>
+int adapters_of(charsiu_gpu *g, const AdaptArgs &a, uint32_t ranks, void *stream)
+{
+	switch (ranks) {
+	case 8: return adapters<T, 8>(g, a, stream);
+	case 16: return adapters<T, 16>(g, a, stream);
+	case 32: return adapters<T, 32>(g, a, stream);
+	case 64: return adapters<T, 64>(g, a, stream);
+	default: return adapters<T, 128>(g, a, stream);
+	}
+}
+
+} // namespace
+
+extern "C" {
+
+int charsiu_gpu_norm_quantise_dev(struct charsiu_gpu *g, const float *x, const float *add,
+				  const float *w, unsigned m, unsigned k, float eps, float *x_out,
+				  int8_t *q, float *d, void *stream)
+{
+	if (!g || layer_dead(g))
+		return -1;
+	if (!x || !w || !q || !d)
+		return refuse(g, "norm_quantise lacks an array");
+	if (!k || k % 32 || k > NORM_ROWS_MAX_K)
+		return refuse(g, "norm_quantise takes rows of a multiple of 32 up to 8192");
+	if (misaligned(x, 16) || misaligned(add, 16) || misaligned(w, 16) || misaligned(x_out, 16) ||
+	    misaligned(q, 16) || misaligned(d, 4))
+		return refuse(g, "norm_quantise: an array is misaligned");
+	if (m > 0x7fffffffu)
+		return refuse(g, "norm_quantise: more rows than a call takes");
+	if (!m)
+		return 0;
+	OnDevice on(g);
+	static uint64_t smem_done;
+	if (!allow_smem(g, norm_rows_kernel, norm_rows_smem(NORM_ROWS_MAX_K), smem_done))
+		return -1;
+	return launch(g, stream, norm_rows_kernel, dim3(m), NORM_ROWS_THREADS, norm_rows_smem(k), x, add, w,
+		      (uint32_t)k, eps, x_out, q, d)
+		       ? 0
+		       : -1;
+}
+
+size_t charsiu_gpu_pages_work(const struct charsiu_gpu_pages *p)
+{
+	return *pages_fault(p) ? 0 : pages_work_words(p->n_pages) * sizeof(int32_t);
+}
+
+int charsiu_gpu_pages_grow_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pages *p,
+			       const int32_t *slots, unsigned n, unsigned add, void *stream)
+{
+	if (slots_check(g, p, slots, n))
+		return -1;
+	if (add > 0x7fffffffu)
+		return refuse(g, "a slot cannot grow that far");
+	if (!n || !add)
+		return 0;
+	OnDevice on(g);
+	return launch(g, stream, pages_grow_kernel, dim3(1), PAGES_PLAN_THREADS, 0, *p, slots,
+		      (uint32_t)n, (uint32_t)add)
+		       ? 0
+		       : -1;
+}
+
+int charsiu_gpu_pages_fork_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pages *p,
+			       const int32_t *from, const int32_t *to, unsigned n, void *stream)
+{
+	if (slots_check(g, p, from, n) || slots_check(g, p, to, n))
+		return -1;
+	if (!n)
+		return 0;
+	OnDevice on(g);
+	return launch(g, stream, pages_fork_plan_kernel, dim3(1), PAGES_PLAN_THREADS, 0, *p, from, to,
+		      (uint32_t)n) &&
+			       launch(g, stream, pages_fork_kernel, dim3(n, 2 * p->n_layer), 256, 0, *p, to)
+		       ? 0
+		       : -1;
+}
+
+int charsiu_gpu_pages_free_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pages *p,
+			       const int32_t *slots, unsigned n, void *stream)
+{
+	if (slots_check(g, p, slots, n))
+		return -1;
+	if (!n)
+		return 0;
+	OnDevice on(g);
+	return launch(g, stream, pages_free_kernel, dim3(n), 128, 0, *p, slots) ? 0 : -1;
+}
+
+int charsiu_gpu_pages_compact_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pages *p,
+				  int32_t *live, void *stream)
+{
+	if (pages_check(g, p, true))
+		return -1;
+	if (misaligned(live, 4))
+		return refuse(g, "an array is misaligned");
+	OnDevice on(g);
+	return launch(g, stream, pages_compact_plan_kernel, dim3(1), PAGES_PLAN_THREADS, 0, *p, live) &&
+			       launch(g, stream, pages_compact_kernel, dim3(8 * layer_sms(g)), 256, 0, *p)
+		       ? 0
+		       : -1;
+}
+
+int charsiu_gpu_pages_append_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pages *p,
+				 unsigned layer, const int32_t *slots, unsigned n, unsigned t,
+				 unsigned n_head, const float *q, const float *k, const float *v,
+				 const float *rope_cs, unsigned n_ctx, void *q_out, void *stream)
+{
+	if (pages_check(g, p, false))
+		return -1;
+	if (layer >= p->n_layer)
+		return refuse(g, "the cache has no such layer");
+	if (!n || !t)
+		return 0;
+	if (!slots || !q || !k || !v || !rope_cs || !q_out)
+		return refuse(g, "append lacks an array");
+	if (!n_head || n_head % p->n_head_kv)
+		return refuse(g, "n_head is no multiple of n_head_kv");
+	if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(rope_cs, 16) ||
+	    misaligned(q_out, 16) || misaligned(slots, 4))
+		return refuse(g, "append: an array is misaligned");
+	if ((uint64_t)n * t > 0x7fffffffull || t > 0x7fffffffu ||
+	    (uint64_t)n * t * (n_head + 2ull * p->n_head_kv) * (p->head_dim / 8) > (0x7fffffffull << 8))
+		return refuse(g, "append: more rows than a call takes");
+	OnDevice on(g);
+	return p->type == TYPE_F16
+		       ? append<__half>(g, p, layer, slots, n, t, n_head, q, k, v, rope_cs, n_ctx, q_out, stream)
+		       : append<__nv_bfloat16>(g, p, layer, slots, n, t, n_head, q, k, v, rope_cs, n_ctx,
+					       q_out, stream);
+}
+
+size_t charsiu_gpu_attention_work(struct charsiu_gpu *g, const struct charsiu_gpu_pages *p,
+				  const struct charsiu_gpu_attention *a)
+{
+	if (!g || *attention_fault(p, a))
+		return 0;
+	return attention_bytes(g, p, a);
+}
+
+int charsiu_gpu_attention_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pages *p,
+			      unsigned layer, const struct charsiu_gpu_attention *b, const void *q,
+			      void *out, void *stream)
+{
+	if (pages_check(g, p, false))
+		return -1;
+	const char *why = attention_fault(p, b);
+	if (*why)
+		return refuse(g, why);
+	if (layer >= p->n_layer)
+		return refuse(g, "the cache has no such layer");
+	if (!b->n_seq)
+		return 0;
+	if (!q || !out || misaligned(q, 16) || misaligned(out, 16) || misaligned(b->slots, 4) ||
+	    misaligned(b->group, 4) || misaligned(b->shared, 4))
+		return refuse(g, "attention: an array is missing or misaligned");
+	AttnArgs a = {};
+	attention_plan(g, p, b, &a);
+	if (!b->work || misaligned(b->work, 16) || b->work_bytes < attention_bytes(g, p, b))
+		return refuse(g, "attention: the work array is missing, misaligned or too small");
+	a.p = *p;
+	a.slots = b->slots;
+	a.group = b->group;
+	a.shared = b->shared;
+	a.q = q;
+	a.out = out;
+	a.part_o = (float *)b->work;
+	a.part_w = a.part_o + (size_t)b->n_seq * b->n_tok * b->n_head * (a.pre_splits + a.own_splits) *
+				      p->head_dim;
+	a.layer = layer;
+	a.n_seq = b->n_seq;
+	a.n_tok = b->n_tok;
+	a.n_head = b->n_head;
+	a.n_group = b->n_group;
+	a.out_type = b->out_type;
+	a.scale = b->scale * 1.4426950408889634f;
+	OnDevice on(g);
+	if (p->type == TYPE_F16)
+		return p->head_dim == 64 ? attention<__half, 64>(g, a, stream)
+					 : attention<__half, 128>(g, a, stream);
+	return p->head_dim == 64 ? attention<__nv_bfloat16, 64>(g, a, stream)
+				 : attention<__nv_bfloat16, 128>(g, a, stream);
+}
+
+size_t charsiu_gpu_adapters_work(struct charsiu_gpu *g, const struct charsiu_gpu_adapters *sets,
+				 unsigned n, unsigned m)
+{
+	return !g || *adapters_fault(sets, n) ? 0 : adapters_bytes(g, sets, n, m);
+}
+
+int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_adapters *sets,
+			     unsigned n, unsigned m, const int8_t *q, const float *d,
+			     const int32_t *which, const float *const *bases, float *const *ys,
+			     void *work, size_t work_bytes, void *stream)
+{
+	if (!g || layer_dead(g))
+		return -1;
+	const char *why = adapters_fault(sets, n);
+	if (*why)
+		return refuse(g, why);
+	if (!m)
+		return 0;
+	if (!q || !d || !which || !ys || misaligned(q, 16) || misaligned(d, 4) || misaligned(which, 4))
+		return refuse(g, "adapters: an array is missing or misaligned");
+	if (m > (1u << 24))
+		return refuse(g, "adapters: more rows than a call takes");
+	if (!work || misaligned(work, 16) || work_bytes < adapters_bytes(g, sets, n, m))
+		return refuse(g, "adapters: the work array is missing, misaligned or too small");
+	AdaptArgs a = {};
+	uint64_t blocks = 0;
+	for (unsigned i = 0; i < n; i++) {
+		AdaptSet &s = a.s[i];
+		s.a = sets[i].a;
+		s.b = sets[i].b;
+		s.rank = sets[i].rank;
+		s.scale = sets[i].scale;
+		s.y = ys[i];
+		s.base = bases ? bases[i] : ys[i];
+		if (!s.y || !s.base || misaligned(s.y, 4) || misaligned(s.base, 4))
+			return refuse(g, "adapters: an output is missing or misaligned");
+		s.n = sets[i].n;
+		s.slots = sets[i].slots;
+		s.max_rank = sets[i].max_rank;
+		blocks += (s.n + ADAPT_COLS - 1) / ADAPT_COLS;
+		s.block_end = (uint32_t)blocks;
+	}
+	if (blocks > 65535)
+		return refuse(g, "adapters: more columns than a call takes");
+	a.q = q;
+	a.d = d;
+	a.which = which;
+	a.t = (float *)work;
+	a.n_sets = n;
+	a.m = m;
+	a.k = sets[0].k;
+	a.pieces = adapters_pieces(g, sets, n, m);
+	a.blocks = (uint32_t)blocks;
+	OnDevice on(g);
+	const uint32_t ranks = adapters_ranks(sets, n);
+	return sets[0].type == TYPE_F16 ? adapters_of<__half>(g, a, ranks, stream)
+					: adapters_of<__nv_bfloat16>(g, a, ranks, stream);
+}
+
+} // extern "C"

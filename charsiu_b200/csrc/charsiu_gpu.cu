@@ -1073,6 +1073,31 @@ void layer_whine(charsiu_gpu *g, const char *why)
 	whine(g, "%s", why);
 }
 
+bool layer_dead(const charsiu_gpu *g)
+{
+	return g->dead;
+}
+
+int layer_sms(const charsiu_gpu *g)
+{
+	return g->sm_count;
+}
+
+cudaStream_t layer_stream(const charsiu_gpu *g)
+{
+	return g->stream;
+}
+
+int *layer_kernel_error(const charsiu_gpu *g)
+{
+	return g->d_err;
+}
+
+void layer_launched(charsiu_gpu *g, unsigned n)
+{
+	g->launches += n;
+}
+
 } // namespace cgpu
 
 // ---- scratch for charsiu_gpu_matvec_batch_noalloc -----------------------------

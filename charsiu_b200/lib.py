@@ -86,6 +86,20 @@ SIGNATURES = [
     ("charsiu_gpu_decoder_generate", C.c_int, [_vp, C.c_int32, C.c_int, C.c_uint, _vp, _vp]),
     ("charsiu_gpu_decoder_launches", C.c_uint, [_vp]),
     ("charsiu_gpu_ordered_sum_dev", C.c_int, [_vp, _vp, C.c_uint, _vp, _vp]),
+    ("charsiu_gpu_norm_quantise_dev", C.c_int, [_vp, _vp, _vp, _vp, C.c_uint, C.c_uint, C.c_float,
+                                                _vp, _vp, _vp, _vp]),
+    ("charsiu_gpu_pages_work", C.c_size_t, [_vp]),
+    ("charsiu_gpu_pages_grow_dev", C.c_int, [_vp, _vp, _vp, C.c_uint, C.c_uint, _vp]),
+    ("charsiu_gpu_pages_fork_dev", C.c_int, [_vp, _vp, _vp, _vp, C.c_uint, _vp]),
+    ("charsiu_gpu_pages_free_dev", C.c_int, [_vp, _vp, _vp, C.c_uint, _vp]),
+    ("charsiu_gpu_pages_compact_dev", C.c_int, [_vp, _vp, _vp, _vp]),
+    ("charsiu_gpu_pages_append_dev", C.c_int, [_vp, _vp, C.c_uint, _vp, C.c_uint, C.c_uint,
+                                               C.c_uint, _vp, _vp, _vp, _vp, C.c_uint, _vp, _vp]),
+    ("charsiu_gpu_attention_work", C.c_size_t, [_vp, _vp, _vp]),
+    ("charsiu_gpu_attention_dev", C.c_int, [_vp, _vp, C.c_uint, _vp, _vp, _vp, _vp]),
+    ("charsiu_gpu_adapters_work", C.c_size_t, [_vp, _vp, C.c_uint, C.c_uint]),
+    ("charsiu_gpu_adapters_dev", C.c_int, [_vp, _vp, C.c_uint, C.c_uint, _vp, _vp, _vp, _vp, _vp,
+                                           _vp, C.c_size_t, _vp]),
     ("charsiu_npu_open", _vp, [C.c_uint, C.c_uint, C.c_uint]),
     ("charsiu_npu_open_ex", _vp, [C.c_uint, C.c_uint, C.c_uint, C.c_int]),
     ("charsiu_npu_close", None, [_vp]),
@@ -126,6 +140,32 @@ def _p(a: np.ndarray) -> int:
 
 class GpuError(RuntimeError):
     pass
+
+
+class PagesStruct(C.Structure):
+    """struct charsiu_gpu_pages: a paged cache in the caller's device memory
+    (pointers are ints, strides in elements)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("len", C.c_void_p),
+                ("ref", C.c_void_p), ("work", C.c_void_p), ("layer_stride", C.c_uint64),
+                ("page_stride", C.c_uint64), ("pos_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("type", C.c_uint32), ("n_layer", C.c_uint32),
+                ("n_pages", C.c_uint32), ("page", C.c_uint32), ("n_head_kv", C.c_uint32),
+                ("head_dim", C.c_uint32), ("n_seq", C.c_uint32), ("max_pages", C.c_uint32)]
+
+
+class AttentionStruct(C.Structure):
+    """struct charsiu_gpu_attention: the batch one attention call is for."""
+    _fields_ = [("slots", C.c_void_p), ("group", C.c_void_p), ("shared", C.c_void_p),
+                ("work", C.c_void_p), ("work_bytes", C.c_size_t), ("n_seq", C.c_uint32),
+                ("n_tok", C.c_uint32), ("n_head", C.c_uint32), ("n_group", C.c_uint32),
+                ("max_len", C.c_uint32), ("out_type", C.c_uint32), ("scale", C.c_float)]
+
+
+class AdaptersStruct(C.Structure):
+    """struct charsiu_gpu_adapters: the low-rank adapters of one projection."""
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("rank", C.c_void_p),
+                ("scale", C.c_void_p), ("k", C.c_uint32), ("n", C.c_uint32),
+                ("slots", C.c_uint32), ("max_rank", C.c_uint32), ("type", C.c_uint32)]
 
 
 class Layer:
@@ -338,6 +378,72 @@ class Layer:
                          stream: int = 0) -> int:
         return self.L.charsiu_gpu_act_quantise_dev(self.h, x_ptr, m, k, q_ptr, d_ptr,
                                                    stream or None)
+
+    # the operators of a batched step: device pointers as ints, structs and
+    # pointer arrays made once by the caller; each raises GpuError if refused
+    def norm_quantise_dev(self, x: int, add: int, w: int, m: int, k: int, eps: float, x_out: int,
+                          q: int, d: int, stream: int = 0):
+        if self.L.charsiu_gpu_norm_quantise_dev(self.h, x, add or None, w, m, k, eps,
+                                                x_out or None, q, d, stream or None):
+            raise GpuError(f"norm_quantise_dev: {self.error()}")
+
+    def pages_work(self, pages: PagesStruct) -> int:
+        """Bytes of pages.work (0: the calls would refuse the cache)."""
+        return self.L.charsiu_gpu_pages_work(C.byref(pages))
+
+    def pages_grow_dev(self, pages: PagesStruct, slots: int, n: int, add: int, stream: int = 0):
+        if self.L.charsiu_gpu_pages_grow_dev(self.h, C.byref(pages), slots, n, add,
+                                             stream or None):
+            raise GpuError(f"pages_grow_dev: {self.error()}")
+
+    def pages_fork_dev(self, pages: PagesStruct, src: int, dst: int, n: int, stream: int = 0):
+        if self.L.charsiu_gpu_pages_fork_dev(self.h, C.byref(pages), src, dst, n, stream or None):
+            raise GpuError(f"pages_fork_dev: {self.error()}")
+
+    def pages_free_dev(self, pages: PagesStruct, slots: int, n: int, stream: int = 0):
+        if self.L.charsiu_gpu_pages_free_dev(self.h, C.byref(pages), slots, n, stream or None):
+            raise GpuError(f"pages_free_dev: {self.error()}")
+
+    def pages_compact_dev(self, pages: PagesStruct, live: int = 0, stream: int = 0):
+        if self.L.charsiu_gpu_pages_compact_dev(self.h, C.byref(pages), live or None,
+                                                stream or None):
+            raise GpuError(f"pages_compact_dev: {self.error()}")
+
+    def pages_append_dev(self, pages: PagesStruct, layer: int, slots: int, n: int, t: int,
+                         n_head: int, q: int, k: int, v: int, rope_cs: int, n_ctx: int,
+                         q_out: int, stream: int = 0):
+        if self.L.charsiu_gpu_pages_append_dev(self.h, C.byref(pages), layer, slots, n, t, n_head,
+                                               q, k, v, rope_cs, n_ctx, q_out, stream or None):
+            raise GpuError(f"pages_append_dev: {self.error()}")
+
+    def attention_work(self, pages: PagesStruct, batch: AttentionStruct) -> int:
+        return self.L.charsiu_gpu_attention_work(self.h, C.byref(pages), C.byref(batch))
+
+    def attention_dev(self, pages: PagesStruct, layer: int, batch: AttentionStruct, q: int,
+                      out: int, stream: int = 0):
+        if self.L.charsiu_gpu_attention_dev(self.h, C.byref(pages), layer, C.byref(batch), q, out,
+                                            stream or None):
+            raise GpuError(f"attention_dev: {self.error()}")
+
+    @staticmethod
+    def adapter_sets(sets):
+        """The AdaptersStructs of a group of projections as the array the calls take."""
+        return (AdaptersStruct * len(sets))(*sets)
+
+    @staticmethod
+    def pointers(ptrs):
+        """Device pointers as the array the calls take."""
+        return (C.c_void_p * len(ptrs))(*ptrs)
+
+    def adapters_work(self, sets, m: int) -> int:
+        return self.L.charsiu_gpu_adapters_work(self.h, sets, len(sets), m)
+
+    def adapters_dev(self, sets, m: int, q: int, d: int, which: int, bases, ys, work: int,
+                     work_bytes: int, stream: int = 0):
+        """sets from adapter_sets; bases (None: in place) and ys from pointers."""
+        if self.L.charsiu_gpu_adapters_dev(self.h, sets, len(sets), m, q, d, which, bases, ys,
+                                           work, work_bytes, stream or None):
+            raise GpuError(f"adapters_dev: {self.error()}")
 
 
 class Llama:

@@ -313,6 +313,180 @@ CHARSIU_GPU_API const float *charsiu_gpu_decoder_logits(const struct charsiu_gpu
 /* kernels one step launches */
 CHARSIU_GPU_API unsigned charsiu_gpu_decoder_launches(const struct charsiu_gpu_decoder *dec);
 
+/* ---- the operators of a batched step ------------------------------------------ */
+/*
+ * What a server that batches sequences runs between its projections
+ * (charsiu_gpu_matvec_batch_group_dev): the norm before them, low-rank adapters
+ * beside them, and a paged cache with the attention that reads it. The manner is
+ * the device-resident forms': device pointers, work queued on `stream` (NULL for
+ * the layer's own), no host synchronisation, no allocation, capturable in a CUDA
+ * graph; 0 when queued, -1 with the reason in charsiu_gpu_error. Every buffer,
+ * scratch included, is the caller's: calls that may run at the same time (two
+ * streams, two captured graphs) need scratch of their own. Arrays that say where
+ * to read or write (slots, tables, adapter numbers) are device memory and are
+ * checked there: an index out of range reads and writes nothing.
+ * No counterpart in the reference, which decodes one token at a time.
+ */
+
+/* rmsnorm of m rows with the residual's addition, and the q8_0 activation of the
+ * result: s = x + add (x alone if add is NULL), q and d what charsiu_act_set
+ * gives of rmsnorm(s) with gains w (src/llama.c:316-326, src/gguf.c:829-882).
+ * Every row is bit-identical to the decode step's. x, add fp32 [m][k], w [k],
+ * q int8 [m][k], d fp32 [m][k/32]; x_out fp32 [m][k] gets s (it may be x or add;
+ * NULL: not wanted). k a multiple of 32, at most 8192; x, add, w, x_out and q
+ * 16-byte aligned, d 4. m 0 does nothing. */
+CHARSIU_GPU_API int charsiu_gpu_norm_quantise_dev(struct charsiu_gpu *g, const float *x,
+						  const float *add, const float *w, unsigned m,
+						  unsigned k, float eps, float *x_out, int8_t *q,
+						  float *d, void *stream);
+
+/* A cache of K and V in pages. All memory is the caller's; pointers are device
+ * pointers. Element (layer, page, position, head, i) of K is
+ * k[layer * layer_stride + page * page_stride + position * pos_stride + head *
+ * head_stride + i] (strides in elements), the same for V: both [page][position]
+ * [head] and [page][head][position] orders can be told. Elements of two
+ * (layer, page, position, head) must not overlap.
+ *
+ * A sequence lives in a slot 0..n_seq-1: len[slot] positions, in the pages
+ * table[slot * max_pages + j], j < ceil(len / page). ref[page] counts the slots
+ * that hold a page; 0 is free. Start with len and ref all 0.
+ *
+ * A call that lists slots takes them in order; one that cannot be done (a slot out
+ * of range or listed before, no room in the table, no free page) is left as it was
+ * and counted in the first int32 of `work`, which only the caller clears. Fresh
+ * pages are the free ones of the lowest numbers, so results never depend on
+ * timing. */
+struct charsiu_gpu_pages {
+	void *k, *v;                       /* 16-byte aligned */
+	int32_t *table;                    /* [n_seq][max_pages] */
+	int32_t *len;                      /* [n_seq] */
+	int32_t *ref;                      /* [n_pages] */
+	int32_t *work;                     /* charsiu_gpu_pages_work bytes, cleared once */
+	uint64_t layer_stride, page_stride, pos_stride, head_stride;   /* multiples of 8 */
+	uint32_t type;                     /* GGML's number: 1 fp16, 30 bf16 */
+	uint32_t n_layer, n_pages;         /* n_pages at most 2^21 */
+	uint32_t page;                     /* positions a page: 16, 32, 64 or 128 */
+	uint32_t n_head_kv, head_dim;      /* head_dim 64 or 128 */
+	uint32_t n_seq, max_pages;
+};
+/* bytes of `work`; 0 for a cache that the calls would refuse */
+CHARSIU_GPU_API size_t charsiu_gpu_pages_work(const struct charsiu_gpu_pages *p);
+/* Slots slots[0..n) grow by `add` positions: len, and the pages for them. Once the
+ * free pages run out at one slot, the later ones that need a page are refused too.
+ * n at most 1024. */
+CHARSIU_GPU_API int charsiu_gpu_pages_grow_dev(struct charsiu_gpu *g,
+					       const struct charsiu_gpu_pages *p,
+					       const int32_t *slots, unsigned n, unsigned add,
+					       void *stream);
+/* Slot to[i] becomes a fork of slot from[i], for i < n <= 1024: it shares the full
+ * pages and gets a copy, in all layers, of the filled positions of a last page that
+ * is not full. to[i] must be empty (len 0). Every source is taken as it was before
+ * the call. Refusals for want of pages as above. */
+CHARSIU_GPU_API int charsiu_gpu_pages_fork_dev(struct charsiu_gpu *g,
+					       const struct charsiu_gpu_pages *p,
+					       const int32_t *from, const int32_t *to, unsigned n,
+					       void *stream);
+/* Slots slots[0..n) become empty; pages that no slot holds any more are free. A
+ * slot listed twice, or empty already, is freed once and not counted as refused. */
+CHARSIU_GPU_API int charsiu_gpu_pages_free_dev(struct charsiu_gpu *g,
+					       const struct charsiu_gpu_pages *p,
+					       const int32_t *slots, unsigned n, void *stream);
+/* Packs the pages in use into 0..live-1: the live pages from `live` on, in order,
+ * go to the free ones below it, in order, in all layers; tables and ref follow.
+ * *live (device, may be NULL) gets their number. */
+CHARSIU_GPU_API int charsiu_gpu_pages_compact_dev(struct charsiu_gpu *g,
+						  const struct charsiu_gpu_pages *p, int32_t *live,
+						  void *stream);
+/* RoPE and the cache's rows, for one layer: row i * t + j of q, k, v (fp32 [n*t]
+ * [heads * head_dim]) is position len - t + j of slot slots[i] (grow the slots
+ * first). q and k are rotated by the position's (cos, sin) pairs of rope_cs
+ * (fp32 [n_ctx][head_dim], as charsiu_gpu_decoder_desc has them), products and
+ * sums in fp32 with the reference's roundings (src/llama.c:364-383), then rounded
+ * once to the cache's type: q to q_out [n*t][n_head][head_dim], k and v into the
+ * pages. A row whose slot, position (negative, or n_ctx and more) or page is out
+ * of range writes nothing. Slots must differ. q, k, v, rope_cs, q_out 16-byte
+ * aligned. */
+CHARSIU_GPU_API int charsiu_gpu_pages_append_dev(struct charsiu_gpu *g,
+						 const struct charsiu_gpu_pages *p, unsigned layer,
+						 const int32_t *slots, unsigned n, unsigned t,
+						 unsigned n_head, const float *q, const float *k,
+						 const float *v, const float *rope_cs,
+						 unsigned n_ctx, void *q_out, void *stream);
+
+/* Attention of a batch over the pages of one layer: n_seq sequences (slots; -1
+ * pads) of n_tok queries each. Query t of sequence i is row i * n_tok + t of q and
+ * stands at position len - n_tok + t of its slot: it sees that position and all
+ * before it. Query head h reads KV head h / (n_head / n_head_kv).
+ *   out = softmax(scale * q K^T) V
+ * with fp32 scores, maxima, sums and accumulators; the weights are rounded to the
+ * cache's type for their product with V, the result once to out_type. A query that
+ * sees nothing (position below 0, an empty or padded slot) gives zeros. What lies
+ * behind a query's position never reaches its result, NaN and inf included.
+ *
+ * Sequences that share their first pages: group g is sequences group[g] to
+ * group[g + 1] - 1 (ascending, device), whose slots hold the same first shared[g]
+ * pages, as charsiu_gpu_pages_fork_dev leaves them. Those pages are then read once
+ * for all of the group's queries. (Only pages that every query of the group sees
+ * whole are taken so; the rest is read through each sequence's own table.)
+ * n_group 0: group and shared may be NULL. Sequences outside all groups share
+ * nothing.
+ *
+ * max_len: about the longest length; results hold for any, the split of the work
+ * over the GPU is chosen by it. */
+struct charsiu_gpu_attention {
+	const int32_t *slots;              /* [n_seq] */
+	const int32_t *group;              /* [n_group + 1] */
+	const int32_t *shared;             /* [n_group], pages */
+	void *work;                        /* charsiu_gpu_attention_work bytes, 16-byte aligned */
+	size_t work_bytes;
+	uint32_t n_seq, n_tok, n_head, n_group;
+	uint32_t max_len;
+	uint32_t out_type;                 /* 0 fp32, or the cache's */
+	float scale;
+};
+/* bytes of `work`, enough for a batch of fewer sequences or groups too; 0 for one
+ * that would be refused */
+CHARSIU_GPU_API size_t charsiu_gpu_attention_work(struct charsiu_gpu *g,
+						  const struct charsiu_gpu_pages *p,
+						  const struct charsiu_gpu_attention *a);
+/* q [n_seq * n_tok][n_head][head_dim] in the cache's type, out the same shape in
+ * out_type; both 16-byte aligned. */
+CHARSIU_GPU_API int charsiu_gpu_attention_dev(struct charsiu_gpu *g,
+					      const struct charsiu_gpu_pages *p, unsigned layer,
+					      const struct charsiu_gpu_attention *a, const void *q,
+					      void *out, void *stream);
+
+/* Low-rank adapters of one projection of K inputs and N outputs: adapter s is
+ * A = a[s] (the first rank[s] rows of [max_rank][K]) and B = b[s] (the first
+ * rank[s] columns of [N][max_rank]), the orders of a GGUF adapter's lora_a and
+ * lora_b. What lies behind rank[s] is not used. Device memory, 16-byte aligned. */
+struct charsiu_gpu_adapters {
+	const void *a;                     /* [slots][max_rank][k] */
+	const void *b;                     /* [slots][n][max_rank] */
+	const int32_t *rank;               /* [slots], 0..max_rank */
+	const float *scale;                /* [slots], alpha / rank */
+	uint32_t k, n;                     /* k a multiple of 32 */
+	uint32_t slots, max_rank;          /* max_rank 4, or a multiple of 8 up to 128 */
+	uint32_t type;                     /* GGML's number: 1 fp16, 30 bf16 */
+};
+/* bytes of scratch for a call of up to m rows; 0 for one that would be refused */
+CHARSIU_GPU_API size_t charsiu_gpu_adapters_work(struct charsiu_gpu *g,
+						 const struct charsiu_gpu_adapters *sets, unsigned n,
+						 unsigned m);
+/* ys[i][r] = bases[i][r] + scale * B (A x_r) of adapter which[r] of sets[i], for the
+ * m rows of the q8_0 activation x = q d that the projections read (q int8 [m][K],
+ * d fp32 [m][K/32]), against n <= 8 sets of the same K. bases and ys: n device
+ * pointers to fp32 [m][N]; bases[i] may be ys[i], and bases NULL means ys: the
+ * projections' outputs get the adapters added. A row whose `which` is no adapter
+ * (-1) is its base. fp32 products and sums throughout. work: 16-byte aligned, as
+ * q is (d 4). */
+CHARSIU_GPU_API int charsiu_gpu_adapters_dev(struct charsiu_gpu *g,
+					     const struct charsiu_gpu_adapters *sets, unsigned n,
+					     unsigned m, const int8_t *q, const float *d,
+					     const int32_t *which, const float *const *bases,
+					     float *const *ys, void *work, size_t work_bytes,
+					     void *stream);
+
 /* ---- accounting ----------------------------------------------------------- */
 
 /* charsiu_npu_submits (include/charsiu_llm.h:197): calls that ran. */
