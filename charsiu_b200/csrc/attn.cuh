@@ -38,16 +38,21 @@ struct AttnArgs {
 	uint32_t pre_splits, own_splits;      // pieces of the prefix and of the rest
 	uint32_t pre_units, own_tiles;        // units of the prefix at most; row tiles a sequence
 	uint32_t out_type;
+	uint32_t beside;      // the prefix is another launch's, before this one: no wait for it
 	float scale;          // scale * log2(e)
+	int *err;             // a wait that gave up says so here
 };
+
+// (Lengths, tables and queries are read past L1: the rows kernel may start without
+// a wait of its own, see there.)
 
 // the length of sequence s of the batch; 0 for a padded one
 __device__ __forceinline__ int32_t attn_len(const AttnArgs &a, uint32_t s)
 {
-	const int32_t slot = a.slots[s];
+	const int32_t slot = __ldcg(&a.slots[s]);
 	if (!pages_slot_ok(a.p, slot))
 		return 0;
-	const int64_t len = a.p.len[slot], most = (int64_t)a.p.max_pages * a.p.page;
+	const int64_t len = __ldcg(&a.p.len[slot]), most = (int64_t)a.p.max_pages * a.p.page;
 	return (int32_t)(len < 0 ? 0 : len > most ? most : len);
 }
 
@@ -62,7 +67,7 @@ struct AttnGroup {
 __device__ __forceinline__ AttnGroup attn_group(const AttnArgs &a, uint32_t g)
 {
 	AttnGroup r;
-	const int32_t b0 = a.group[g], b1 = a.group[g + 1];
+	const int32_t b0 = __ldcg(&a.group[g]), b1 = __ldcg(&a.group[g + 1]);
 	r.s0 = b0 < 0 ? 0 : b0 > (int32_t)a.n_seq ? a.n_seq : (uint32_t)b0;
 	r.s1 = b1 < (int32_t)r.s0 ? r.s0 : b1 > (int32_t)a.n_seq ? a.n_seq : (uint32_t)b1;
 	int32_t least = 0x7fffffff;
@@ -79,11 +84,11 @@ __device__ __forceinline__ AttnGroup attn_group(const AttnArgs &a, uint32_t g)
 	r.keys = 0;
 	r.slot = -1;
 	if (first != 0xffffffffu && least > 0) {
-		int32_t pages = a.shared[g];
+		int32_t pages = __ldcg(&a.shared[g]);
 		pages = min(pages, (int32_t)a.p.max_pages);
 		pages = min(pages, least / (int32_t)a.p.page);
 		r.keys = pages > 0 ? pages * (int32_t)a.p.page : 0;
-		r.slot = a.slots[first];
+		r.slot = __ldcg(&a.slots[first]);
 	}
 	return r;
 }
@@ -93,7 +98,8 @@ __device__ __forceinline__ AttnGroup attn_group_of(const AttnArgs &a, uint32_t s
 {
 	for (uint32_t g0 = 0; g0 < a.n_group; g0 += 32) {
 		const uint32_t g = g0 + (threadIdx.x & 31);
-		const bool in = g < a.n_group && a.group[g] <= (int32_t)s && (int32_t)s < a.group[g + 1];
+		const bool in = g < a.n_group && __ldcg(&a.group[g]) <= (int32_t)s &&
+				(int32_t)s < __ldcg(&a.group[g + 1]);
 		const uint32_t who = __ballot_sync(0xffffffffu, in);
 		if (who)
 			return attn_group(a, g0 + __ffs(who) - 1);
@@ -115,8 +121,8 @@ __device__ __forceinline__ bool attn_find_unit(const AttnArgs &a, uint32_t u, ui
 	for (uint32_t g0 = 0; g0 < a.n_group; g0 += 32) {
 		uint32_t n = 0;
 		if (g0 + lane < a.n_group) {
-			const int32_t b0 = max(a.group[g0 + lane], 0);
-			const int32_t b1 = min(a.group[g0 + lane + 1], (int32_t)a.n_seq);
+			const int32_t b0 = max(__ldcg(&a.group[g0 + lane]), 0);
+			const int32_t b1 = min(__ldcg(&a.group[g0 + lane + 1]), (int32_t)a.n_seq);
 			if (b1 > b0)
 				n = ((uint32_t)(b1 - b0) * a.n_tok * a.gqa + rows - 1) / rows;
 		}
@@ -236,7 +242,19 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a)
 	constexpr int NT = HD / 8, KS = HD / 16;
 	const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa;
-	pdl_wait();
+	// Beside the prefix's launch this one starts once all of that one's CTAs are past
+	// their own wait, so what came before both is done; what it writes, that one
+	// does not touch. It ends after that one, as the join counts on.
+	struct EndAfter {
+		bool late;
+		__device__ ~EndAfter()
+		{
+			if (late)
+				pdl_wait();
+		}
+	} end_after{a.beside != 0};
+	if (!a.beside)
+		pdl_wait();
 	pdl_launch_dependents();
 
 	// which rows, which keys
@@ -274,7 +292,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a)
 		k1 = attn_len(a, s0);
 		if (k1 == 0)
 			return;
-		slot = a.slots[s0];
+		slot = __ldcg(&a.slots[s0]);
 		k0 = attn_group_of(a, s0).keys;
 		attn_piece(k0, k1, piece, a.own_splits, ATTN_GRAIN);
 		slot_at = a.pre_splits + piece;
@@ -308,7 +326,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
 		for (int j = 0; j < 4; j++) {
 			const T *src = qp[j & 1];
-			qa[ks][j] = src ? *(const uint32_t *)(src + ks * 16 + (j >> 1) * 8 + c * 2) : 0u;
+			qa[ks][j] = src ? __ldcg((const uint32_t *)(src + ks * 16 + (j >> 1) * 8 + c * 2)) : 0u;
 		}
 
 	float o[NT][4];
@@ -332,7 +350,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a)
 			bool ok = pos < k1;
 			int32_t page = 0;
 			if (ok) {
-				page = row[pos / a.p.page];
+				page = __ldcg(&row[pos / a.p.page]);
 				ok = (uint32_t)page < a.p.n_pages;
 				page = ok ? page : 0;
 			}

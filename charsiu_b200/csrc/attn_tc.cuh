@@ -1,0 +1,445 @@
+// SPDX-License-Identifier: GPL-2.0-or-later
+// The shared prefix of a group on the tensor cores (tcgen05): up to 256 rows
+// (queries of one KV head: sequence, token, head of the group) against one piece of
+// the prefix's keys, one CTA.
+//
+// With r rows sharing K and V, a key costs 4 r hd operations for its 4 hd bytes: at
+// 256 rows the tensor cores and HBM are about balanced, and the softmax's r
+// exponentials a key (16 a cycle and multiprocessor) cost as much as the products
+// of hd = 128. So the three must overlap:
+//
+//   warp 9      copies K and V tiles of 128 keys, page by page, by tensor copies
+//               (128-byte swizzle) into a ring
+//   warp 8      issues the MMAs: S = Q K^T (M = 128 rows, N = 128 keys) into tensor
+//               memory, and O += P V with P read from tensor memory, where
+//               it lies over the S it was made of, and V as an operand whose N
+//               (hd) is the contiguous side
+//   warps 0-7   two streams of 128 rows, a thread a row: scores out of tensor
+//               memory, maximum, exponentials, the sum, P back
+//
+// While one stream is in its exponentials the tensor cores work for the other. With
+// more than 128 rows in the unit the streams are its two halves; with fewer they
+// are the same rows over the even and the odd tiles of keys, joined with the other
+// pieces at the end.
+//
+// O is scaled only where a row's maximum has grown by more than 2^8 since it was
+// last taken (P stays below 2^8, exact enough in both types); the weight of the
+// piece is taken with the same maximum, so the result is the same.
+#pragma once
+
+#include <cuda.h>
+
+#include "attn.cuh"
+#include "tcgen05.cuh"
+
+namespace cgpu {
+
+constexpr uint32_t ATC_KEYS = 128, ATC_ROWS = 256;
+constexpr int ATC_THREADS = 320;
+constexpr uint32_t ATC_SLAB = ATC_KEYS * 128;        // 128 rows of 64 elements
+
+// Tiles in the ring: what fits beside Q
+template <int HD>
+__host__ __device__ constexpr uint32_t atc_ring()
+{
+	return HD == 128 ? 5 : 10;
+}
+
+template <int HD>
+constexpr size_t atc_smem()
+{
+	return 1024 + ((size_t)ATC_ROWS + atc_ring<HD>() * ATC_KEYS) * HD * 2;
+}
+
+// K-major or N-major operand, 128-byte swizzle (8 rows of 128 bytes an atom): `lbo`
+// the distance between 64-element columns of atoms (N-major), `sbo` between 8-row
+// groups. Version 1 (sm_100).
+__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo)
+{
+	return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)((lbo >> 4) & 0x3fffu) << 16) |
+	       ((uint64_t)((sbo >> 4) & 0x3fffu) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// dense kind::f16 MMA, D fp32, M = 128: A and B both fp16 (0) or both bf16 (1); B
+// N-major where b_mn
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t bf16, uint32_t n, bool b_mn)
+{
+	return (1u << 4) | (bf16 << 7) | (bf16 << 10) | ((uint32_t)b_mn << 16) | ((n >> 3) << 17) |
+	       ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+					   bool accumulate)
+{
+	asm volatile("{\n\t.reg .pred p;\n\t"
+		     "setp.ne.b32 p, %4, 0;\n\t"
+		     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+		     :: "r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+
+// A from tensor memory: 16 bits a value, two a word, a row a lane
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
+					   bool accumulate)
+{
+	asm volatile("{\n\t.reg .pred p;\n\t"
+		     "setp.ne.b32 p, %4, 0;\n\t"
+		     "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+		     :: "r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+
+// 32 lanes x 32 consecutive columns
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *r)
+{
+	uint32_t *u = reinterpret_cast<uint32_t *>(r);
+	asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+		     "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+		     "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+		     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
+		       "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]),
+		       "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
+		       "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+		       "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]),
+		       "=r"(u[31])
+		     : "r"(taddr));
+}
+
+// The wait for such loads does not name their registers, so nothing would keep the
+// compiler from using them before it: this makes them its results.
+__device__ __forceinline__ void tmem_loaded32(float *r)
+{
+	uint32_t *u = reinterpret_cast<uint32_t *>(r);
+#pragma unroll
+	for (int i = 0; i < 32; i += 8)
+		asm volatile("" : "+r"(u[i]), "+r"(u[i + 1]), "+r"(u[i + 2]), "+r"(u[i + 3]), "+r"(u[i + 4]),
+				  "+r"(u[i + 5]), "+r"(u[i + 6]), "+r"(u[i + 7]));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *u)
+{
+	asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+		     "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+		     "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+		     :: "r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
+		     "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]),
+		     "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]),
+		     "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]),
+		     "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+		     : "memory");
+}
+
+// a box of (64 elements, positions of a page) of one head of one page
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, int x, int y, int z, int w,
+					    uint64_t *bar)
+{
+	asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+		     " [%0], [%1, {%2, %3, %4, %5}], [%6];"
+		     :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+		     : "memory");
+}
+
+// codes of a wait that gave up, after the batched matvec's (5 to 13)
+constexpr int ATC_ERR_RING = 21, ATC_ERR_MMA = 22, ATC_ERR_ROWS = 23;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(ATC_THREADS, 1)
+attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+	       const __grid_constant__ CUtensorMap vmap)
+{
+	constexpr uint32_t NB = atc_ring<HD>(), SLABS = HD / 64, TILE = ATC_KEYS * HD * 2;
+	constexpr uint32_t COL_S = 0, COL_O = 256;      // S (and P) 128 columns a stream, then O
+	extern __shared__ uint8_t atc_raw[];
+	__shared__ __align__(8) uint64_t b_full[NB], b_free[NB], b_q, b_s[2], b_p[2], b_o[2], b_end;
+	__shared__ uint32_t s_tmem;
+	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	const uint32_t q_at = (smem_addr(atc_raw) + 1023u) & ~1023u, ring = q_at + ATC_ROWS * HD * 2;
+	uint8_t *q_ptr = atc_raw + (q_at - smem_addr(atc_raw));
+	pdl_wait();
+	pdl_launch_dependents();
+
+	// which rows, which keys (every warp for itself)
+	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa, splits = a.pre_splits / 2;
+	uint32_t b = blockIdx.x;
+	const uint32_t u = b / (kvh_n * splits);
+	b -= u * kvh_n * splits;
+	const uint32_t piece = b / kvh_n, kvh = b - piece * kvh_n;
+	uint32_t g, tile;
+	if (!attn_find_unit(a, u, ATC_ROWS, &g, &tile))
+		return;
+	const AttnGroup gr = attn_group(a, g);
+	if (!gr.keys)
+		return;
+	int32_t k0 = 0, k1 = gr.keys;
+	attn_piece(k0, k1, piece, splits, ATC_KEYS);
+	const uint32_t n_rows = (gr.s1 - gr.s0) * tg, row0 = tile * ATC_ROWS;
+	const bool halves = n_rows - row0 > 128;
+	const uint32_t tiles = (uint32_t)(k1 - k0 + (int32_t)ATC_KEYS - 1) / ATC_KEYS;
+	const uint32_t pieces = a.pre_splits + a.own_splits;
+	// row r of the unit: its place in q, and in the pieces
+	auto row_of = [&](uint32_t r) {
+		const uint32_t s = gr.s0 + r / tg, x = r % tg;
+		return (size_t)(s * a.n_tok + x / a.gqa) * a.n_head + kvh * a.gqa + x % a.gqa;
+	};
+	if (!tiles) {
+		for (uint32_t r = row0 + threadIdx.x; r < min(row0 + ATC_ROWS, n_rows); r += ATC_THREADS) {
+			a.part_w[row_of(r) * pieces + 2 * piece] = -INFINITY;
+			a.part_w[row_of(r) * pieces + 2 * piece + 1] = -INFINITY;
+		}
+		return;
+	}
+	// the tiles of stream i
+	auto count = [&](uint32_t i) { return halves ? tiles : (tiles + 1 - i) / 2; };
+
+	if (warp == 8) {
+		if (lane == 0) {
+			for (uint32_t i = 0; i < NB; i++) {
+				mbar_init(&b_full[i], 1);
+				mbar_init(&b_free[i], 1);
+			}
+			mbar_init(&b_q, 256);
+			mbar_init(&b_end, 1);
+			for (int i = 0; i < 2; i++) {
+				mbar_init(&b_s[i], 1);
+				mbar_init(&b_p[i], 128);
+				mbar_init(&b_o[i], 1);
+			}
+			fence_mbar_init();
+		}
+		__syncwarp();
+		tmem_alloc(&s_tmem, 512);
+		tmem_relinquish();
+	}
+	tc_fence_before();
+	__syncthreads();
+	tc_fence_after();
+	const uint32_t tmem = s_tmem;
+
+	if (warp == 9) {
+		// ---- K and V tiles into the ring: K of tile j is copy 2 j, V copy 2 j + 1
+		const uint32_t per = ATC_KEYS / a.p.page;        // pages a tile
+		const int32_t *row = a.p.table + (size_t)gr.slot * a.p.max_pages + k0 / (int32_t)a.p.page;
+		const uint32_t left = (uint32_t)(k1 - k0) / a.p.page;      // pages of the piece
+		const uint32_t my_page = lane % per, my_slab = lane / per;
+		bool ok = true;
+		uint32_t c = 0;
+		for (uint32_t j = 0; j < tiles && ok; j++) {
+			// a page past the piece, or no page at all, reads as zeros
+			int32_t page = (int32_t)a.p.n_pages;
+			if (j * per + my_page < left) {
+				page = __ldcg(&row[j * per + my_page]);
+				page = (uint32_t)page < a.p.n_pages ? page : (int32_t)a.p.n_pages;
+			}
+			for (int v = 0; v < 2; v++, c++) {
+				const uint32_t at = c % NB;
+				if (c >= NB)
+					ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_free[at], (c / NB - 1) & 1,
+										       WAIT_LIMIT_NS));
+				if (!ok)
+					break;
+				if (lane == 0)
+					mbar_arrive_expect_tx(&b_full[at], TILE);
+				__syncwarp();
+				if (my_slab < SLABS)
+					tma_load_4d(ring + at * TILE + my_slab * ATC_SLAB + my_page * a.p.page * 128,
+						    v ? &vmap : &kmap, (int)(my_slab * 64), 0, (int)kvh, page,
+						    &b_full[at]);
+				__syncwarp();
+			}
+		}
+		// every copy issued lands before the CTA leaves (already so unless a wait gave up)
+		if (!ok && lane == 0)
+			*(volatile int *)a.err = ATC_ERR_RING;
+		for (uint32_t i = c > NB ? c - NB : 0; i < c; i++)
+			if (!mbar_wait_bounded(&b_full[i % NB], (i / NB) & 1, WAIT_LIMIT_NS) && lane == 0)
+				*(volatile int *)a.err = ATC_ERR_RING;
+	} else if (warp == 8) {
+		if (lane == 0) {
+			// ---- the MMAs
+			constexpr uint32_t BF = std::is_same<T, __nv_bfloat16>::value;
+			constexpr uint32_t id_s = idesc_f16(BF, ATC_KEYS, false), id_o = idesc_f16(BF, HD, true);
+			bool ok = mbar_wait_bounded(&b_q, 0, WAIT_LIMIT_NS);
+			tc_fence_after();
+			auto scores = [&](uint32_t i, uint32_t n) {      // S of stream i's n-th tile
+				const uint32_t j = halves ? n : 2 * n + i, c = 2 * j, at = c % NB;
+				ok = ok && mbar_wait_bounded(&b_full[at], (c / NB) & 1, WAIT_LIMIT_NS);
+				if (!ok)
+					return;
+				tc_fence_after();
+				const uint32_t qa = q_at + (halves ? i * 128 * 128 : 0), ka = ring + at * TILE;
+#pragma unroll
+				for (uint32_t k = 0; k < HD / 16; k++)
+					mma_f16_ss(tmem + COL_S + i * 128,
+						   smem_desc_sw128(qa + (k / 4) * (ATC_ROWS * 128) + (k % 4) * 32, 16, 1024),
+						   smem_desc_sw128(ka + (k / 4) * ATC_SLAB + (k % 4) * 32, 16, 1024), id_s,
+						   k != 0);
+				mma_commit(&b_s[i]);
+				if (!halves || i == 1)
+					mma_commit(&b_free[at]);
+			};
+			auto outputs = [&](uint32_t i, uint32_t n) {     // O += P V of the same
+				const uint32_t j = halves ? n : 2 * n + i, c = 2 * j + 1, at = c % NB;
+				ok = ok && mbar_wait_bounded(&b_full[at], (c / NB) & 1, WAIT_LIMIT_NS) &&
+				     mbar_wait_bounded(&b_p[i], n & 1, WAIT_LIMIT_NS);
+				if (!ok)
+					return;
+				tc_fence_after();
+				const uint32_t va = ring + at * TILE;
+#pragma unroll
+				for (uint32_t k = 0; k < ATC_KEYS / 16; k++)
+					mma_f16_ts(tmem + COL_O + i * HD, tmem + COL_S + i * 128 + k * 8,
+						   smem_desc_sw128(va + k * 16 * 128, ATC_SLAB, 1024), id_o, n || k);
+				mma_commit(&b_o[i]);
+				if (!halves || i == 1)
+					mma_commit(&b_free[at]);
+			};
+			const uint32_t n0 = count(0), n1 = count(1);
+			scores(0, 0);
+			if (n1)
+				scores(1, 0);
+			for (uint32_t n = 0; n < n0 && ok; n++) {
+				outputs(0, n);
+				if (n + 1 < n0)
+					scores(0, n + 1);
+				if (n < n1)
+					outputs(1, n);
+				if (n + 1 < n1)
+					scores(1, n + 1);
+			}
+			// all MMAs done before tensor memory is freed
+			mma_commit(&b_end);
+			if (!mbar_wait_bounded(&b_end, 0, WAIT_LIMIT_NS) || !ok)
+				*(volatile int *)a.err = ATC_ERR_MMA;
+		}
+		__syncwarp();
+	} else {
+		// ---- rows: Q into shared memory first (swizzled as the tensor copies would)
+		const uint32_t rows = halves ? 256 : 128;
+		const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;     // scale > 0 from here on
+		for (uint32_t x = threadIdx.x; x < rows * (HD / 8); x += 256) {
+			const uint32_t r = x / (HD / 8), w = x % (HD / 8);
+			uint4 v = make_uint4(0, 0, 0, 0);
+			if (row0 + r < n_rows)
+				v = *(const uint4 *)((const T *)a.q + row_of(row0 + r) * HD + w * 8);
+			v.x ^= flip;
+			v.y ^= flip;
+			v.z ^= flip;
+			v.w ^= flip;
+			*(uint4 *)(q_ptr + (w / 8) * (ATC_ROWS * 128) + r * 128 + (((w % 8) ^ (r & 7)) << 4)) = v;
+		}
+		fence_proxy_async_smem();
+		mbar_arrive(&b_q);
+
+		const uint32_t i = warp / 4, quarter = warp % 4, mine = count(i);
+		const uint32_t lanes = (quarter * 32) << 16;
+		const uint32_t ts = tmem + lanes + COL_S + i * 128, to = tmem + lanes + COL_O + i * HD;
+		const float scale = fabsf(a.scale);
+		float m = -INFINITY, l = 0.0f;
+		bool ok = true;
+		for (uint32_t n = 0; n < mine; n++) {
+			ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_s[i], n & 1, WAIT_LIMIT_NS));
+			if (!ok)
+				break;
+			tc_fence_after();
+			float s[128];
+#pragma unroll
+			for (int c = 0; c < 4; c++)
+				tmem_ld32(ts + 32 * c, s + 32 * c);
+			tmem_wait_ld();
+#pragma unroll
+			for (int c = 0; c < 4; c++)
+				tmem_loaded32(s + 32 * c);
+			const int32_t in_tile = k1 - k0 - (int32_t)((halves ? n : 2 * n + i) * ATC_KEYS);
+			if (in_tile < (int32_t)ATC_KEYS) {
+#pragma unroll
+				for (int c = 0; c < 128; c++)
+					if (c >= in_tile)
+						s[c] = -INFINITY;
+			}
+			float mx[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+			for (int c = 0; c < 128; c++)
+				mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+			mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+			if (n == 0) {
+				m = mx[0];
+			} else if (__any_sync(0xffffffffu, (mx[0] - m) * scale > 8.0f)) {
+				const float f = mx[0] == m ? 1.0f : exp2_approx((m - mx[0]) * scale);
+				ok = __all_sync(0xffffffffu,
+						mbar_wait_bounded(&b_o[i], (n - 1) & 1, WAIT_LIMIT_NS));
+				if (!ok)
+					break;
+				tc_fence_after();
+#pragma unroll 1
+				for (int c = 0; c < HD / 32; c++) {
+					float o[32];
+					tmem_ld32(to + 32 * c, o);
+					tmem_wait_ld();
+					tmem_loaded32(o);
+#pragma unroll
+					for (int e = 0; e < 32; e++)
+						o[e] *= f;
+					tmem_st32(to + 32 * c, reinterpret_cast<uint32_t *>(o));
+				}
+				l *= f;
+				m = mx[0];
+			}
+			const float base = m == -INFINITY ? 0.0f : -m * scale;
+			float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+				uint32_t w[32];
+#pragma unroll
+				for (int c = 0; c < 32; c++) {
+					const float x = exp2_approx(__fmaf_rn(s[64 * h + 2 * c], scale, base));
+					const float y = exp2_approx(__fmaf_rn(s[64 * h + 2 * c + 1], scale, base));
+					sum[0] += x;
+					sum[1] += y;
+					w[c] = pack_pair<T>(x, y);
+				}
+				tmem_st32(ts + 32 * h, w);
+			}
+			l += sum[0] + sum[1];
+			tmem_wait_st();
+			tc_fence_before();
+			mbar_arrive(&b_p[i]);
+		}
+		if (ok && mine)
+			ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_o[i], (mine - 1) & 1, WAIT_LIMIT_NS));
+		if (!ok && lane == 0)
+			*(volatile int *)a.err = ATC_ERR_ROWS;
+		if (ok) {
+			tc_fence_after();
+			const uint32_t r = row0 + (halves ? i * 128 : 0) + quarter * 32 + lane;
+			const bool real = r < n_rows;
+			const size_t at = real ? row_of(r) * pieces + 2 * piece + (halves ? 0 : i) : 0;
+			const float inv = l != 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
+			if (real) {
+				a.part_w[at] = l != 0.0f ? (m == -INFINITY ? 0.0f : m * scale) + log2f(l) : -INFINITY;
+				if (halves)
+					a.part_w[at + 1] = -INFINITY;
+			}
+			if (mine) {
+#pragma unroll 1
+				for (int c = 0; c < HD / 32; c++) {
+					float o[32];
+					tmem_ld32(to + 32 * c, o);
+					tmem_wait_ld();
+					tmem_loaded32(o);
+					if (real)
+#pragma unroll
+						for (int e = 0; e < 32; e += 4)
+							*(float4 *)(a.part_o + at * HD + 32 * c + e) =
+								make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv,
+									    o[e + 3] * inv);
+				}
+			}
+		}
+		tc_fence_before();
+	}
+	__syncthreads();
+	if (warp == 8) {
+		tc_fence_after();
+		tmem_dealloc(tmem, 512);
+	}
+}
+
+} // namespace cgpu

@@ -6,6 +6,7 @@
 // Every launch has the programmatic attribute, and every kernel waits for its
 // predecessor before it reads or writes anything of the caller's.
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>          // PFN_cuTensorMapEncodeTiled
 
 #include <cstdio>
 #include <type_traits>
@@ -14,6 +15,7 @@
 
 #include "adapters.cuh"
 #include "attn.cuh"
+#include "attn_tc.cuh"
 #include "layer_internal.h"
 #include "norm_rows.cuh"
 #include "pages.cuh"
@@ -178,58 +180,94 @@ const char *attention_fault(const charsiu_gpu_pages *p, const charsiu_gpu_attent
 
 constexpr uint32_t ATTN_CTAS_PER_SM = 3, ATTN_MAX_SPLITS = 32;
 
-// How the work is cut.
-void attention_plan(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gpu_attention *b,
+// How the work is cut. Returns whether the prefixes go to the tensor cores.
+bool attention_plan(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gpu_attention *b,
 		    AttnArgs *a)
 {
 	const uint32_t gqa = b->n_head / p->n_head_kv, rows = b->n_tok * gqa;
 	const uint32_t sms = (uint32_t)layer_sms(g);
+	const uint64_t all = (uint64_t)b->n_seq * rows;
+	auto splits = [&](uint64_t ctas, uint64_t aim, uint64_t pieces) {
+		uint64_t n = ctas ? aim / ctas : 1;
+		n = n > ATTN_MAX_SPLITS ? ATTN_MAX_SPLITS : n < 1 ? 1 : n;
+		return (uint32_t)(n < pieces ? n : pieces);
+	};
 	a->gqa = gqa;
 	a->own_tiles = (rows + ATTN_TILE_ROWS - 1) / ATTN_TILE_ROWS;
-	a->pre_units = b->n_group ? (uint32_t)(((uint64_t)b->n_seq * rows + ATTN_TILE_ROWS - 1) /
-					       ATTN_TILE_ROWS) + b->n_group
-				  : 0;
-	const uint32_t grains = (b->max_len + ATTN_GRAIN - 1) / ATTN_GRAIN + 1;
-	auto splits = [&](uint64_t ctas) {
-		uint64_t n = ctas ? ((uint64_t)ATTN_CTAS_PER_SM * sms + ctas - 1) / ctas : 1;
-		n = n > ATTN_MAX_SPLITS ? ATTN_MAX_SPLITS : n < 1 ? 1 : n;
-		return (uint32_t)(n < grains ? n : grains);
-	};
-	a->own_splits = splits((uint64_t)b->n_seq * a->own_tiles * p->n_head_kv);
-	a->pre_splits = b->n_group ? splits((uint64_t)a->pre_units * p->n_head_kv) : 0;
+	a->own_splits = splits((uint64_t)b->n_seq * a->own_tiles * p->n_head_kv, ATTN_CTAS_PER_SM * sms,
+			       b->max_len / ATTN_GRAIN + 1);
+	a->pre_units = a->pre_splits = 0;
+	if (!b->n_group)
+		return false;
+	const bool tc = all >= 32;
+	const uint32_t unit = tc ? ATC_ROWS : ATTN_TILE_ROWS;
+	a->pre_units = (uint32_t)((all + unit - 1) / unit);
+	a->pre_splits = tc ? 2 * splits((uint64_t)a->pre_units * p->n_head_kv, sms, b->max_len / ATC_KEYS + 1)
+			   : splits((uint64_t)a->pre_units * p->n_head_kv, ATTN_CTAS_PER_SM * sms,
+				    b->max_len / ATTN_GRAIN + 1);
+	a->pre_units += b->n_group;          // each group may end in a part of a unit
+	return tc;
 }
 
 // Scratch for the pieces of this batch and of any smaller one: fewer sequences are
-// cut finer, but n sequences of c CTAs each give at most n + target / c pieces of
+// cut finer, but n sequences of c CTAs each give at most n + aim / c pieces of
 // each kind, which grows with n.
 size_t attention_bytes(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gpu_attention *b)
 {
 	const uint64_t kv = p->n_head_kv, n = b->n_seq, rows = (uint64_t)b->n_tok * (b->n_head / kv);
 	const uint64_t tiles = (rows + ATTN_TILE_ROWS - 1) / ATTN_TILE_ROWS, most = ATTN_MAX_SPLITS * n;
-	const uint64_t target = ATTN_CTAS_PER_SM * (uint64_t)layer_sms(g);
-	uint64_t parts = n + target / (tiles * kv) + 1;
+	const uint64_t sms = (uint64_t)layer_sms(g);
+	uint64_t parts = n + ATTN_CTAS_PER_SM * sms / (tiles * kv) + 1;
 	parts = parts < most ? parts : most;
 	if (b->n_group) {
-		const uint64_t pre = n + target * ATTN_TILE_ROWS / (rows * kv) + 1;
-		parts += pre < most ? pre : most;
+		const uint64_t pre = 2 * (n + sms * ATC_ROWS / (rows * kv) + 1);
+		parts += pre < 2 * most ? pre : 2 * most;
 	}
 	return (size_t)(parts * b->n_tok * b->n_head * (p->head_dim + 1) * sizeof(float) + 15) / 16 * 16;
 }
 
-template <typename T, int HD>
-int attention(charsiu_gpu *g, const AttnArgs &a, void *stream)
+// K or V of one layer as (element, position, head, page); boxes of 64 elements and a
+// page's positions. A dimension of one element has no stride to speak of.
+bool attention_map(CUtensorMap *map, const charsiu_gpu_pages *p, const void *base, unsigned layer)
 {
-	static uint64_t smem_done;
+	const auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encode());
+	if (!enc)
+		return false;
+	const cuuint64_t dims[4] = {p->head_dim, p->page, p->n_head_kv, p->n_pages};
+	const cuuint64_t row = 2ull * p->head_dim;
+	const cuuint64_t strides[3] = {2 * p->pos_stride, p->n_head_kv > 1 ? 2 * p->head_stride : row,
+				       p->n_pages > 1 ? 2 * p->page_stride : row};
+	const cuuint32_t box[4] = {64, p->page, 1, 1}, ones[4] = {1, 1, 1, 1};
+	return enc(map, p->type == TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+		   4, (uint8_t *)const_cast<void *>(base) + 2 * layer * p->layer_stride, dims, strides, box, ones,
+		   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+		   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD>
+int attention(charsiu_gpu *g, AttnArgs &a, bool tc, void *stream)
+{
+	static uint64_t smem_done, tc_done;
 	if (!allow_smem(g, attn_rows_kernel<T, HD>, attn_rows_smem<HD>(), smem_done))
 		return -1;
-	const uint64_t blocks = (uint64_t)a.p.n_head_kv *
-				((uint64_t)a.pre_units * a.pre_splits +
-				 (uint64_t)a.n_seq * a.own_tiles * a.own_splits);
-	if (blocks > 0x7fffffffull)
+	const uint64_t pre = (uint64_t)a.p.n_head_kv * a.pre_units * (tc ? a.pre_splits / 2 : a.pre_splits);
+	const uint64_t own = (uint64_t)a.p.n_head_kv * a.n_seq * a.own_tiles * a.own_splits;
+	if (pre + own > 0x7fffffffull)
 		return refuse(g, "the batch is larger than the call takes");
+	if (tc) {
+		CUtensorMap kmap, vmap;
+		if (!attention_map(&kmap, &a.p, a.p.k, a.layer) || !attention_map(&vmap, &a.p, a.p.v, a.layer))
+			return refuse(g, "the cache's strides cannot be described to the copy engine");
+		if (!allow_smem(g, attn_tc_kernel<T, HD>, atc_smem<HD>(), tc_done) ||
+		    !launch(g, stream, attn_tc_kernel<T, HD>, dim3((unsigned)pre), ATC_THREADS, atc_smem<HD>(), a,
+			    kmap, vmap))
+			return -1;
+		a.pre_units = 0;
+		a.beside = 1;
+	}
 	const uint64_t rows = (uint64_t)a.n_seq * a.n_tok * a.n_head;
-	return launch(g, stream, attn_rows_kernel<T, HD>, dim3((unsigned)blocks), ATTN_WARPS * 32,
-		      attn_rows_smem<HD>(), a) &&
+	return launch(g, stream, attn_rows_kernel<T, HD>, dim3((unsigned)(own + (tc ? 0 : pre))),
+		      ATTN_WARPS * 32, attn_rows_smem<HD>(), a) &&
 			       launch(g, stream, attn_join_kernel<T, HD>,
 				      dim3((unsigned)((rows + 7) / 8)), 256, 0, a)
 		       ? 0
@@ -455,7 +493,7 @@ int charsiu_gpu_attention_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pa
 	    misaligned(b->group, 4) || misaligned(b->shared, 4))
 		return refuse(g, "attention: an array is missing or misaligned");
 	AttnArgs a = {};
-	attention_plan(g, p, b, &a);
+	const bool tc = attention_plan(g, p, b, &a);
 	if (!b->work || misaligned(b->work, 16) || b->work_bytes < attention_bytes(g, p, b))
 		return refuse(g, "attention: the work array is missing, misaligned or too small");
 	a.p = *p;
@@ -474,12 +512,13 @@ int charsiu_gpu_attention_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pa
 	a.n_group = b->n_group;
 	a.out_type = b->out_type;
 	a.scale = b->scale * 1.4426950408889634f;
+	a.err = layer_kernel_error(g);
 	OnDevice on(g);
 	if (p->type == TYPE_F16)
-		return p->head_dim == 64 ? attention<__half, 64>(g, a, stream)
-					 : attention<__half, 128>(g, a, stream);
-	return p->head_dim == 64 ? attention<__nv_bfloat16, 64>(g, a, stream)
-				 : attention<__nv_bfloat16, 128>(g, a, stream);
+		return p->head_dim == 64 ? attention<__half, 64>(g, a, tc, stream)
+					 : attention<__half, 128>(g, a, tc, stream);
+	return p->head_dim == 64 ? attention<__nv_bfloat16, 64>(g, a, tc, stream)
+				 : attention<__nv_bfloat16, 128>(g, a, tc, stream);
 }
 
 size_t charsiu_gpu_adapters_work(struct charsiu_gpu *g, const struct charsiu_gpu_adapters *sets,

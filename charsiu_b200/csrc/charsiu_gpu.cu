@@ -1098,6 +1098,11 @@ void layer_launched(charsiu_gpu *g, unsigned n)
 	g->launches += n;
 }
 
+void *tensor_map_encode()
+{
+	return reinterpret_cast<void *>(tensor_map_encoder());
+}
+
 } // namespace cgpu
 
 // ---- scratch for charsiu_gpu_matvec_batch_noalloc -----------------------------

@@ -22,5 +22,6 @@ int layer_sms(const charsiu_gpu *g);
 cudaStream_t layer_stream(const charsiu_gpu *g);
 int *layer_kernel_error(const charsiu_gpu *g);   // the device word a wait that gave up writes
 void layer_launched(charsiu_gpu *g, unsigned n);
+void *tensor_map_encode();      // the driver's cuTensorMapEncodeTiled, or null
 
 } // namespace cgpu
