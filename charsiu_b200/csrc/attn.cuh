@@ -13,8 +13,11 @@
 // joins the pieces: o = sum_j w_j o_j, w_j proportional to the weights.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "charsiu_gpu.h"
 #include "pages.cuh"
@@ -24,8 +27,9 @@ namespace cgpu {
 
 constexpr uint32_t ATTN_TILE_ROWS = 16;      // rows of a unit: the m of mma.m16n8k16
 constexpr uint32_t ATTN_WARPS = 4;
-constexpr uint32_t ATTN_KEYS = 32;           // keys a warp takes at a time
-constexpr uint32_t ATTN_GRAIN = ATTN_WARPS * ATTN_KEYS;
+constexpr uint32_t ATTN_GRAIN = 128;         // keys: pieces are cut to multiples of it
+constexpr uint32_t ATTN_MAX_SPLITS = 32;     // pieces of a sequence's own keys; of a prefix twice as many
+constexpr uint32_t ATTN_MAX_PIECES = 3 * ATTN_MAX_SPLITS;
 
 struct AttnArgs {
 	charsiu_gpu_pages p;
@@ -36,7 +40,9 @@ struct AttnArgs {
 	float *part_w;        // [row][pieces]: log2 of the piece's weight, -inf: nothing in it
 	uint32_t layer, n_seq, n_tok, n_head, n_group, gqa;
 	uint32_t pre_splits, own_splits;      // pieces of the prefix and of the rest
+	uint32_t own_grain;                   // keys: the least a piece of the rest has
 	uint32_t pre_units, own_tiles;        // units of the prefix at most; row tiles a sequence
+	uint32_t rows_splits;                 // pieces of the prefix that the rows kernel makes
 	uint32_t out_type;
 	uint32_t beside;      // the prefix is another launch's, before this one: no wait for it
 	float scale;          // scale * log2(e)
@@ -194,13 +200,6 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
 		     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-// 16 bytes global -> shared, or zeros (nothing is read then)
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void *gmem, bool ok)
-{
-	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-		     :: "r"(smem), "l"(gmem), "r"(ok ? 16 : 0) : "memory");
-}
-
 __device__ __forceinline__ float exp2_approx(float x)
 {
 	float y;
@@ -221,314 +220,464 @@ __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v)
 	return __bfloat162float(v);
 }
 
+// ---- rows of 16 ----------------------------------------------------------------------
+//
+// Items of work: 16 rows (queries of one KV head: sequence, token, head of the group)
+// against one piece of keys, of a sequence's own or of a prefix. Bound by memory:
+// a key's K and V serve few rows, so what counts is that enough of them are on
+// their way at all times. Each of a persistent grid's CTAs takes items in turn; one
+// warp runs ahead through its items (lengths, tables, then tensor copies of K and
+// V page by page, and of the item's queries) into a ring of stages, so the latency
+// of one item's start hides behind the work on the ones before. Four warps take a
+// quarter of a stage's keys each (mma.m16n8k16, scores and outputs in registers,
+// one pass with a running maximum and sum) and are joined through the item's last
+// stage before it is given back.
 template <int HD>
-constexpr size_t attn_rows_smem()
+struct AttnRing {
+	static constexpr uint32_t KEYS = HD == 128 ? 64 : 128;      // a stage's; 32 KB of K and V
+	static constexpr uint32_t WKEYS = KEYS / ATTN_WARPS;        // a warp's
+	static constexpr uint32_t STAGES = 3;
+	static constexpr uint32_t SLAB = KEYS * 128;                // 64 elements of each key
+	static constexpr uint32_t HALF = KEYS * HD * 2;             // K, then V
+	static constexpr uint32_t Q_ROW = HD * 2 + 16;              // (16 bytes on: other banks)
+	static constexpr uint32_t Q_AT = 2 * HALF;
+	static constexpr uint32_t STAGE = (Q_AT + ATTN_TILE_ROWS * Q_ROW + 1023) / 1024 * 1024;
+	static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE;
+};
+
+struct AttnStage {
+	uint32_t kind;        // 1: an item's first stage, 2: its last, 4: no keys at all, 8: the end,
+			      // 16: of a prefix, 32: its rows have no prefix
+	uint32_t s0, n_rows, tile, kvh, slot_at;
+	int32_t key0, k1;     // the stage's first key; the piece's end
+	int32_t len;          // the sequence's length (a prefix is seen whole)
+};
+
+// a box of (64 elements, positions of a page) of one head of one page
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, int x, int y, int z, int w,
+					    uint64_t *bar)
 {
-	return (size_t)ATTN_WARPS * 2 * 2 * ATTN_KEYS * HD * 2;      // warps, stages, K and V
+	asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+		     " [%0], [%1, {%2, %3, %4, %5}], [%6];"
+		     :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+		     : "memory");
 }
 
-// 16 rows (queries of one KV head: sequence, token, head of the group) against one
-// piece of keys. Four warps, each with 32-key tiles of its own (every fourth) that
-// it copies to shared memory two deep; scores, weights and outputs stay in
-// registers; the warps' results are joined at the end. Shared rows are swizzled
-// by 16-byte words (word ^ (key & 7)), so ldmatrix meets no bank conflict.
+constexpr int ATTN_THREADS = (ATTN_WARPS + 1) * 32;
+// codes of a wait that gave up, after the batched matvec's (5 to 13)
+constexpr int ATTN_ERR_RING = 24, ATTN_ERR_ROWS = 25;
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(ATTN_WARPS * 32)
-attn_rows_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(ATTN_THREADS)
+attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+		 const __grid_constant__ CUtensorMap vmap)
 {
-	extern __shared__ __align__(128) uint8_t asm_[];
-	__shared__ float s_m[ATTN_WARPS][ATTN_TILE_ROWS], s_l[ATTN_WARPS][ATTN_TILE_ROWS];
-	constexpr int KW = HD / 8;                       // 16-byte words a key
+	using R = AttnRing<HD>;
+	constexpr uint32_t NS = R::STAGES;
 	constexpr int NT = HD / 8, KS = HD / 16;
-	const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa;
+	extern __shared__ uint8_t rows_raw[];
+	__shared__ __align__(8) uint64_t b_full[NS], b_free[NS];
+	__shared__ __align__(8) uint64_t b_join;
+	__shared__ AttnStage s_stage[NS];
+	__shared__ float s_m[ATTN_WARPS][ATTN_TILE_ROWS], s_l[ATTN_WARPS][ATTN_TILE_ROWS];
+	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	const uint32_t ring = (smem_addr(rows_raw) + 1023u) & ~1023u;
+	uint8_t *ring_ptr = rows_raw + (ring - smem_addr(rows_raw));
+	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa, pieces = a.pre_splits + a.own_splits;
+	if (threadIdx.x == 0) {
+		for (uint32_t i = 0; i < NS; i++) {
+			mbar_init(&b_full[i], 1);
+			mbar_init(&b_free[i], ATTN_WARPS);
+		}
+		mbar_init(&b_join, ATTN_WARPS);
+		fence_mbar_init();
+	}
+	__syncthreads();
 	// Beside the prefix's launch this one starts once all of that one's CTAs are past
 	// their own wait, so what came before both is done; what it writes, that one
 	// does not touch. It ends after that one, as the join counts on.
-	struct EndAfter {
-		bool late;
-		__device__ ~EndAfter()
-		{
-			if (late)
-				pdl_wait();
-		}
-	} end_after{a.beside != 0};
 	if (!a.beside)
 		pdl_wait();
 	pdl_launch_dependents();
+	const uint32_t pre_items = a.pre_units * kvh_n * a.rows_splits;
+	const uint32_t own_items = a.n_seq * a.own_tiles * kvh_n * a.own_splits, items = pre_items + own_items;
 
-	// which rows, which keys
-	uint32_t b = blockIdx.x, s0, s1, tile, piece, kvh, slot_at;
-	int32_t k0, k1, slot;
-	const uint32_t pre_blocks = a.pre_units * kvh_n * a.pre_splits;
-	if (b < pre_blocks) {
-		const uint32_t u = b / (kvh_n * a.pre_splits);
-		b -= u * kvh_n * a.pre_splits;
-		piece = b / kvh_n;
-		kvh = b - piece * kvh_n;
-		uint32_t g;
-		if (!attn_find_unit(a, u, ATTN_TILE_ROWS, &g, &tile))
-			return;
-		const AttnGroup gr = attn_group(a, g);
-		if (!gr.keys)
-			return;
-		s0 = gr.s0;
-		s1 = gr.s1;
-		slot = gr.slot;
-		k0 = 0;
-		k1 = gr.keys;
-		attn_piece(k0, k1, piece, a.pre_splits, ATTN_GRAIN);
-		slot_at = piece;
+	if (warp == ATTN_WARPS) {
+		// ---- the items, and their K, V and queries into the ring
+		const uint32_t box = min(a.p.page, 64u), row_bytes = HD * 2;
+		uint32_t c = 0;
+		bool ok = true;
+		AttnGroup gr = {1, 0, 0, -1};           // the last group looked up: sequences [s0, s1)
+		auto push = [&](AttnStage h, const int32_t *row) {
+			const uint32_t st = c % NS, base = ring + st * R::STAGE;
+			if (c >= NS)
+				ok = __all_sync(0xffffffffu,
+						mbar_wait_bounded(&b_free[st], (c / NS - 1) & 1, WAIT_LIMIT_NS));
+			if (!ok)
+				return;
+			uint32_t boxes = 0;
+			if (!(h.kind & 4)) {
+				const uint32_t keys = min((uint32_t)(h.k1 - h.key0), R::KEYS);
+				boxes = (keys + box - 1) / box;
+			}
+			const uint32_t q_rows = (h.kind & 5) == 1 ? min(h.n_rows - h.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS) : 0;
+			// this lane's box: which positions, which 64 elements; K and V alike
+			const uint32_t mine = lane % (R::KEYS / 16), slab = lane / (R::KEYS / 16);
+			const uint32_t pos = (uint32_t)h.key0 + mine * box;
+			int page = (int)a.p.n_pages;            // (no page: zeros)
+			if (mine < boxes && slab < HD / 64) {
+				const uint32_t id = (uint32_t)__ldcg(&row[pos / a.p.page]);
+				page = (int)min(id, a.p.n_pages);
+			}
+			if (lane == 0) {
+				s_stage[st] = h;
+				mbar_arrive_expect_tx(&b_full[st], 2 * boxes * box * row_bytes + q_rows * row_bytes);
+			}
+			__syncwarp();
+			if (mine < boxes && slab < HD / 64) {
+				const uint32_t dst = base + slab * R::SLAB + mine * box * 128;
+				tma_load_4d(dst, &kmap, (int)(slab * 64), (int)(pos % a.p.page), (int)h.kvh, page,
+					    &b_full[st]);
+				tma_load_4d(dst + R::HALF, &vmap, (int)(slab * 64), (int)(pos % a.p.page), (int)h.kvh,
+					    page, &b_full[st]);
+			}
+			if (lane < q_rows) {
+				const uint32_t r = h.tile * ATTN_TILE_ROWS + lane, s = h.s0 + r / tg, x = r % tg;
+				const T *src = (const T *)a.q + ((size_t)(s * a.n_tok + x / a.gqa) * a.n_head +
+								 h.kvh * a.gqa + x % a.gqa) * HD;
+				bulk_g2s(ring_ptr + st * R::STAGE + R::Q_AT + lane * R::Q_ROW, src, row_bytes,
+					 &b_full[st]);
+			}
+			__syncwarp();
+			c++;
+		};
+		for (uint32_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
+			AttnStage h;
+			int32_t k0, slot;
+			uint32_t b = it, kind = 0;
+			if (b < pre_items) {
+				const uint32_t u = b / (kvh_n * a.rows_splits);
+				b -= u * kvh_n * a.rows_splits;
+				const uint32_t piece = b / kvh_n;
+				h.kvh = b - piece * kvh_n;
+				uint32_t g;
+				if (!attn_find_unit(a, u, ATTN_TILE_ROWS, &g, &h.tile))
+					continue;
+				gr = attn_group(a, g);
+				if (!gr.keys)
+					continue;
+				h.s0 = gr.s0;
+				h.n_rows = (gr.s1 - gr.s0) * tg;
+				slot = gr.slot;
+				k0 = 0;
+				h.k1 = gr.keys;
+				attn_piece(k0, h.k1, piece, a.rows_splits, ATTN_GRAIN);
+				h.slot_at = piece;
+				h.len = 0x7fffffff;
+				kind = 16;
+			} else {
+				b -= pre_items;
+				const uint32_t per = a.own_tiles * kvh_n * a.own_splits;
+				h.s0 = b / per;
+				b -= h.s0 * per;
+				h.tile = b / (kvh_n * a.own_splits);
+				b -= h.tile * kvh_n * a.own_splits;
+				const uint32_t piece = b / kvh_n;
+				h.kvh = b - piece * kvh_n;
+				h.n_rows = tg;
+				if (h.s0 < gr.s0 || h.s0 >= gr.s1)
+					gr = attn_group_of(a, h.s0);
+				h.k1 = h.len = attn_len(a, h.s0);
+				slot = __ldcg(&a.slots[h.s0]);
+				k0 = h.k1 ? gr.keys : 0;
+				kind = !piece && !k0 ? 32 : 0;          // (the first piece says so for its rows)
+				attn_piece(k0, h.k1, piece, a.own_splits, a.own_grain);
+				h.slot_at = a.pre_splits + piece;
+			}
+			if (k0 >= h.k1) {
+				h.kind = kind | 7;
+				h.key0 = k0;
+				push(h, nullptr);
+				continue;
+			}
+			const int32_t *row = a.p.table + (size_t)slot * a.p.max_pages;
+			for (int32_t key0 = k0; key0 < h.k1 && ok; key0 += (int32_t)R::KEYS) {
+				h.kind = kind | (key0 == k0 ? 1u : 0u) | (key0 + (int32_t)R::KEYS >= h.k1 ? 2u : 0u);
+				h.key0 = key0;
+				push(h, row);
+			}
+		}
+		// the end; then every copy issued lands before the CTA leaves
+		AttnStage end = {};
+		end.kind = 8 | 4;
+		if (ok)
+			push(end, nullptr);
+		if (!ok && lane == 0)
+			*(volatile int *)a.err = ATTN_ERR_RING;
+		for (uint32_t i = c > NS ? c - NS : 0; i < c; i++)
+			if (!mbar_wait_bounded(&b_full[i % NS], (i / NS) & 1, WAIT_LIMIT_NS) && lane == 0)
+				*(volatile int *)a.err = ATTN_ERR_RING;
 	} else {
-		b -= pre_blocks;
-		const uint32_t per = a.own_tiles * kvh_n * a.own_splits;
-		s0 = b / per;
-		b -= s0 * per;
-		tile = b / (kvh_n * a.own_splits);
-		b -= tile * kvh_n * a.own_splits;
-		piece = b / kvh_n;
-		kvh = b - piece * kvh_n;
-		s1 = s0 + 1;
-		k1 = attn_len(a, s0);
-		if (k1 == 0)
-			return;
-		slot = __ldcg(&a.slots[s0]);
-		k0 = attn_group_of(a, s0).keys;
-		attn_piece(k0, k1, piece, a.own_splits, ATTN_GRAIN);
-		slot_at = a.pre_splits + piece;
-	}
-	const uint32_t n_rows = (s1 - s0) * tg, pieces = a.pre_splits + a.own_splits;
-
-	// this thread's two rows of the accumulators: lane / 4 and 8 more
-	int32_t limit[2];
-	const T *qp[2];
-	const uint32_t c = lane & 3;
-#pragma unroll
-	for (int h = 0; h < 2; h++) {
-		const uint32_t r = tile * ATTN_TILE_ROWS + lane / 4 + 8 * h;
-		limit[h] = k1;
-		qp[h] = nullptr;
-		if (r < n_rows) {
-			const uint32_t s = s0 + r / tg, t = r % tg / a.gqa;
-			const int32_t len = attn_len(a, s);
-			if (len > 0)
-				limit[h] = len - (int32_t)a.n_tok + (int32_t)t + 1;
-			qp[h] = (const T *)a.q + ((size_t)(s * a.n_tok + t) * a.n_head + kvh * a.gqa +
-						  r % a.gqa) * HD;
-		}
-	}
-	const int32_t least = min(min(__reduce_min_sync(0xffffffffu, limit[0]),
-				      __reduce_min_sync(0xffffffffu, limit[1])), k1);
-
-	uint32_t qa[KS][4];
-#pragma unroll
-	for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-		for (int j = 0; j < 4; j++) {
-			const T *src = qp[j & 1];
-			qa[ks][j] = src ? __ldcg((const uint32_t *)(src + ks * 16 + (j >> 1) * 8 + c * 2)) : 0u;
-		}
-
-	float o[NT][4];
-	float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-	for (int n = 0; n < NT; n++)
-		o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-
-	constexpr uint32_t TILE_BYTES = ATTN_KEYS * HD * 2;
-	uint8_t *stage0 = asm_ + (size_t)warp * 4 * TILE_BYTES;
-	const T *kbase = (const T *)a.p.k + a.layer * a.p.layer_stride + kvh * a.p.head_stride;
-	const T *vbase = (const T *)a.p.v + a.layer * a.p.layer_stride + kvh * a.p.head_stride;
-	const int32_t *row = a.p.table + (size_t)slot * a.p.max_pages;
-
-	auto load = [&](int st, int32_t key0) {
-		const uint32_t ks = smem_addr(stage0 + st * 2 * TILE_BYTES), vs = ks + TILE_BYTES;
-#pragma unroll
-		for (int it = 0; it < (int)ATTN_KEYS * KW / 32; it++) {
-			const uint32_t key = it * (32 / KW) + lane / KW, w = lane % KW;
-			const int32_t pos = key0 + (int32_t)key;
-			bool ok = pos < k1;
-			int32_t page = 0;
-			if (ok) {
-				page = __ldcg(&row[pos / a.p.page]);
-				ok = (uint32_t)page < a.p.n_pages;
-				page = ok ? page : 0;
+		// ---- rows
+		const uint32_t q4 = lane & 3;
+		uint32_t qa[KS][4];
+		float o[NT][4], m[2], l[2];
+		int32_t limit[2], least = 0;
+		uint32_t joins = 0;
+		bool ended = false;
+		auto together = [&]() {                 // the four warps, as a barrier that can give up
+			__syncwarp();
+			if (lane == 0)
+				mbar_arrive(&b_join);
+			return (bool)__all_sync(0xffffffffu, mbar_wait_bounded(&b_join, joins++ & 1, WAIT_LIMIT_NS));
+		};
+		for (uint32_t c = 0;; c++) {
+			const uint32_t st = c % NS;
+			if (!__all_sync(0xffffffffu, mbar_wait_bounded(&b_full[st], (c / NS) & 1, WAIT_LIMIT_NS)))
+				break;
+			const AttnStage h = s_stage[st];
+			if (h.kind & 8) {
+				ended = true;
+				break;
 			}
-			const uint64_t off = page * a.p.page_stride +
-					     (uint32_t)(pos % a.p.page) * a.p.pos_stride + w * 8;
-			const uint32_t dst = key * HD * 2 + ((w ^ (key & 7)) << 4);
-			cp_async16_or_zero(ks + dst, kbase + off, ok);
-			cp_async16_or_zero(vs + dst, vbase + off, ok);
-		}
-		asm volatile("cp.async.commit_group;" ::: "memory");
-	};
-
-	const int32_t first = k0 + (int32_t)(warp * ATTN_KEYS), step = (int32_t)ATTN_GRAIN;
-	if (first < k1)
-		load(0, first);
-	int st = 0;
-	for (int32_t key0 = first; key0 < k1; key0 += step, st ^= 1) {
-		if (key0 + step < k1) {
-			load(st ^ 1, key0 + step);
-			asm volatile("cp.async.wait_group 1;" ::: "memory");
-		} else {
-			asm volatile("cp.async.wait_group 0;" ::: "memory");
-		}
-		__syncwarp();
-		const uint32_t ks = smem_addr(stage0 + st * 2 * TILE_BYTES), vs = ks + TILE_BYTES;
-		float s[4][4];
+			if (h.kind & 1) {
+				m[0] = m[1] = -INFINITY;
+				l[0] = l[1] = 0.0f;
 #pragma unroll
-		for (int j = 0; j < 4; j++) {
-			s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-			const uint32_t key = j * 8 + (lane & 7);
-#pragma unroll
-			for (int k2 = 0; k2 < KS / 2; k2++) {
-				uint32_t kb[4];
-				ldmatrix_x4(kb, ks + key * HD * 2 + (((k2 * 4 + lane / 8) ^ (key & 7)) << 4));
-				mma_16816<T>(s[j], qa[2 * k2], kb[0], kb[1]);
-				mma_16816<T>(s[j], qa[2 * k2 + 1], kb[2], kb[3]);
+				for (int n = 0; n < NT; n++)
+					o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 			}
-		}
-		const bool ragged = key0 + (int32_t)ATTN_KEYS > least;
-		float mx[2] = {m[0], m[1]};
+			if ((h.kind & 5) == 1) {
+				// this thread's rows of the accumulators: lane / 4 and 8 more
 #pragma unroll
-		for (int j = 0; j < 4; j++)
-#pragma unroll
-			for (int e = 0; e < 4; e++) {
-				s[j][e] *= a.scale;
-				if (ragged && key0 + j * 8 + (int32_t)c * 2 + (e & 1) >= min(limit[e >> 1], k1))
-					s[j][e] = -INFINITY;
-				mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
-			}
-#pragma unroll
-		for (int h = 0; h < 2; h++) {
-			mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-			mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-			const float base = mx[h] == -INFINITY ? 0.0f : mx[h];
-			const float keep = exp2_approx(m[h] - base);
-			m[h] = mx[h];
-			l[h] *= keep;
-#pragma unroll
-			for (int n = 0; n < NT; n++) {
-				o[n][2 * h] *= keep;
-				o[n][2 * h + 1] *= keep;
-			}
-#pragma unroll
-			for (int j = 0; j < 4; j++) {
-				s[j][2 * h] = exp2_approx(s[j][2 * h] - base);
-				s[j][2 * h + 1] = exp2_approx(s[j][2 * h + 1] - base);
-				l[h] += s[j][2 * h] + s[j][2 * h + 1];
-			}
-		}
-		// A weight of 0 must take nothing from its key, and 0 * inf is NaN: where
-		// some row of the tile does not see some key that others do, V is
-		// searched for inf and NaN, and such a tile goes key by key.
-		bool plain = true;
-		if (ragged && key0 + (int32_t)ATTN_KEYS > least && least < k1) {
-			bool bad = false;
-			for (uint32_t w = lane; w < TILE_BYTES / 4; w += 32) {
-				uint32_t two;
-				asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(vs + w * 4) : "memory");
-				const uint32_t e = sizeof(T) && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-				bad |= (two & e) == e || ((two >> 16) & e) == e;
-			}
-			plain = !__any_sync(0xffffffffu, bad);
-		}
-		if (plain) {
-#pragma unroll
-			for (int k16 = 0; k16 < 2; k16++) {
-				const uint32_t pa[4] = {pack_pair<T>(s[2 * k16][0], s[2 * k16][1]),
-							pack_pair<T>(s[2 * k16][2], s[2 * k16][3]),
-							pack_pair<T>(s[2 * k16 + 1][0], s[2 * k16 + 1][1]),
-							pack_pair<T>(s[2 * k16 + 1][2], s[2 * k16 + 1][3])};
-				const uint32_t key = k16 * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-#pragma unroll
-				for (int n2 = 0; n2 < NT / 2; n2++) {
-					uint32_t vb[4];
-					ldmatrix_x4_trans(vb, vs + key * HD * 2 +
-							  (((n2 * 2 + (lane >> 4)) ^ (key & 7)) << 4));
-					mma_16816<T>(o[2 * n2], pa, vb[0], vb[1]);
-					mma_16816<T>(o[2 * n2 + 1], pa, vb[2], vb[3]);
+				for (int e = 0; e < 2; e++) {
+					const uint32_t r = h.tile * ATTN_TILE_ROWS + lane / 4 + 8 * e;
+					limit[e] = r < h.n_rows ? h.len - (int32_t)a.n_tok + (int32_t)(r % tg / a.gqa) + 1
+								: h.k1;
 				}
+				least = min(min(__reduce_min_sync(0xffffffffu, limit[0]),
+						__reduce_min_sync(0xffffffffu, limit[1])), h.k1);
+				const uint32_t rows = min(h.n_rows - h.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS);
+				const uint8_t *qs = ring_ptr + st * R::STAGE + R::Q_AT;
+#pragma unroll
+				for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+					for (int j = 0; j < 4; j++) {
+						const uint32_t r = lane / 4 + 8 * (j & 1);
+						qa[ks][j] = r < rows ? *(const uint32_t *)(qs + r * R::Q_ROW + ks * 32 +
+											   (j >> 1) * 16 + q4 * 4)
+								     : 0u;
+					}
 			}
-		} else {
+			const uint32_t ks_ = ring + st * R::STAGE, vs = ks_ + R::HALF, w0 = warp * R::WKEYS;
+			const int32_t key0 = h.key0 + (int32_t)w0;
+			if (!(h.kind & 4) && key0 < h.k1) {
+				constexpr int NK = R::WKEYS / 8;
+				float s[NK][4];
+#pragma unroll
+				for (int j = 0; j < NK; j++) {
+					s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+					const uint32_t key = w0 + j * 8 + (lane & 7);
+#pragma unroll
+					for (int k2 = 0; k2 < KS / 2; k2++) {
+						const uint32_t w = k2 * 4 + lane / 8;
+						uint32_t kb[4];
+						ldmatrix_x4(kb, ks_ + (w / 8) * R::SLAB + key * 128 + (((w % 8) ^ (key & 7)) << 4));
+						mma_16816<T>(s[j], qa[2 * k2], kb[0], kb[1]);
+						mma_16816<T>(s[j], qa[2 * k2 + 1], kb[2], kb[3]);
+					}
+				}
+				const bool ragged = key0 + (int32_t)R::WKEYS > least;
+				float mx[2] = {m[0], m[1]};
+#pragma unroll
+				for (int j = 0; j < NK; j++)
+#pragma unroll
+					for (int e = 0; e < 4; e++) {
+						s[j][e] *= a.scale;
+						if (ragged && key0 + j * 8 + (int32_t)q4 * 2 + (e & 1) >= min(limit[e >> 1], h.k1))
+							s[j][e] = -INFINITY;
+						mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
+					}
+#pragma unroll
+				for (int e = 0; e < 2; e++) {
+					mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+					mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+				}
+				if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
+#pragma unroll
+					for (int e = 0; e < 2; e++) {
+						const float keep = mx[e] == m[e] ? 1.0f : exp2_approx(m[e] - mx[e]);
+						m[e] = mx[e];
+						l[e] *= keep;
+#pragma unroll
+						for (int n = 0; n < NT; n++) {
+							o[n][2 * e] *= keep;
+							o[n][2 * e + 1] *= keep;
+						}
+					}
+				}
+#pragma unroll
+				for (int e = 0; e < 2; e++) {
+					const float base = m[e] == -INFINITY ? 0.0f : m[e];
+#pragma unroll
+					for (int j = 0; j < NK; j++) {
+						s[j][2 * e] = exp2_approx(s[j][2 * e] - base);
+						s[j][2 * e + 1] = exp2_approx(s[j][2 * e + 1] - base);
+						l[e] += s[j][2 * e] + s[j][2 * e + 1];
+					}
+				}
+				// A weight of 0 must take nothing from its key, and 0 * inf is NaN. Keys
+				// behind the piece's end are cleared; where some row does not see some
+				// key that others do, V is searched for inf and NaN, and such a tile
+				// goes key by key.
+				bool plain = true;
+				if (ragged && key0 + (int32_t)R::WKEYS > h.k1) {
+					const uint32_t end = (uint32_t)(h.k1 - key0);
+					for (uint32_t x = lane; x < (R::WKEYS - end) * (HD / 8); x += 32) {
+						const uint32_t key = w0 + end + x / (HD / 8), w = x % (HD / 8);
+						asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};"
+							     :: "r"(vs + (w / 8) * R::SLAB + key * 128 + (w % 8) * 16), "r"(0)
+							     : "memory");
+					}
+					fence_proxy_async_smem();
+					__syncwarp();
+				}
+				if (ragged && least < h.k1) {
+					bool bad = false;
+					for (uint32_t x = lane; x < R::WKEYS * (HD / 2); x += 32) {
+						const uint32_t key = w0 + x / (HD / 2), w = x % (HD / 2);
+						uint32_t two;
+						asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two)
+							     : "r"(vs + (w / 32) * R::SLAB + key * 128 + (w % 32) * 4) : "memory");
+						const uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+						bad |= (two & e) == e || ((two >> 16) & e) == e;
+					}
+					plain = !__any_sync(0xffffffffu, bad);
+				}
+				if (plain) {
+#pragma unroll
+					for (int k16 = 0; k16 < NK / 2; k16++) {
+						const uint32_t pa[4] = {pack_pair<T>(s[2 * k16][0], s[2 * k16][1]),
+									pack_pair<T>(s[2 * k16][2], s[2 * k16][3]),
+									pack_pair<T>(s[2 * k16 + 1][0], s[2 * k16 + 1][1]),
+									pack_pair<T>(s[2 * k16 + 1][2], s[2 * k16 + 1][3])};
+						const uint32_t key = w0 + k16 * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+						for (int n2 = 0; n2 < NT / 2; n2++) {
+							const uint32_t w = n2 * 2 + (lane >> 4);
+							uint32_t vb[4];
+							ldmatrix_x4_trans(vb, vs + (w / 8) * R::SLAB + key * 128 +
+									  (((w % 8) ^ (key & 7)) << 4));
+							mma_16816<T>(o[2 * n2], pa, vb[0], vb[1]);
+							mma_16816<T>(o[2 * n2 + 1], pa, vb[2], vb[3]);
+						}
+					}
+				} else {
 #pragma unroll 1
-			for (int key = 0; key < (int)ATTN_KEYS; key++) {
-				float w[2];
+					for (int key = 0; key < (int)R::WKEYS; key++) {
+						float w[2];
 #pragma unroll
-				for (int h = 0; h < 2; h++) {
-					float x = 0.0f;
+						for (int e = 0; e < 2; e++) {
+							float x = 0.0f;
 #pragma unroll
-					for (int j = 0; j < 4; j++)
-						if (key / 8 == j)
-							x = key & 1 ? s[j][2 * h + 1] : s[j][2 * h];
-					w[h] = to_float<T>(T(__shfl_sync(0xffffffffu, x, (lane & ~3u) + (key % 8) / 2)));
-				}
+							for (int j = 0; j < NK; j++)
+								if (key / 8 == j)
+									x = key & 1 ? s[j][2 * e + 1] : s[j][2 * e];
+							w[e] = to_float<T>(T(__shfl_sync(0xffffffffu, x, (lane & ~3u) + (key % 8) / 2)));
+						}
+						const uint32_t kk = w0 + key;
 #pragma unroll
-				for (int n = 0; n < NT; n++) {
-					uint32_t two;
-					asm volatile("ld.shared.u32 %0, [%1];"
-						     : "=r"(two)
-						     : "r"(vs + key * HD * 2 + ((n ^ (key & 7)) << 4) + c * 4)
-						     : "memory");
-					T v[2];
-					*(uint32_t *)v = two;
+						for (int n = 0; n < NT; n++) {
+							uint32_t two;
+							asm volatile("ld.shared.u32 %0, [%1];"
+								     : "=r"(two)
+								     : "r"(vs + (n / 8) * R::SLAB + kk * 128 +
+									   (((n % 8) ^ (kk & 7)) << 4) + q4 * 4)
+								     : "memory");
+							T v[2];
+							*(uint32_t *)v = two;
 #pragma unroll
-					for (int e = 0; e < 4; e++)
-						if (key0 + key < min(limit[e >> 1], k1))
-							o[n][e] = __fmaf_rn(w[e >> 1], to_float<T>(v[e & 1]), o[n][e]);
+							for (int e = 0; e < 4; e++)
+								if (key0 + key < min(limit[e >> 1], h.k1))
+									o[n][e] = __fmaf_rn(w[e >> 1], to_float<T>(v[e & 1]), o[n][e]);
+						}
+					}
 				}
 			}
+			if (h.kind & 2) {
+				// the warps joined: maxima and sums, then the outputs through this stage
+				const uint32_t row0 = h.tile * ATTN_TILE_ROWS;
+				const uint32_t rows = min(h.n_rows - row0, ATTN_TILE_ROWS);
+#pragma unroll
+				for (int e = 0; e < 2; e++) {
+					l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+					l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+					if (q4 == 0) {
+						s_m[warp][lane / 4 + 8 * e] = m[e];
+						s_l[warp][lane / 4 + 8 * e] = l[e];
+					}
+				}
+				if (!together())                           // all have read the stage
+					break;
+				float *os = reinterpret_cast<float *>(ring_ptr + st * R::STAGE);     // [warps][16][HD]
+#pragma unroll
+				for (int e = 0; e < 2; e++)
+					if (lane / 4 + 8 * e < rows)
+#pragma unroll
+						for (int n = 0; n < NT; n++)
+							*(float2 *)(os + (warp * ATTN_TILE_ROWS + lane / 4 + 8 * e) * HD +
+								    ((n * 8) ^ ((lane / 4 & 3) * 8)) + q4 * 2) =
+								make_float2(o[n][2 * e], o[n][2 * e + 1]);
+				if (!together())
+					break;
+				for (uint32_t x = threadIdx.x; x < rows * (HD / 4); x += ATTN_WARPS * 32) {
+					const uint32_t r = x / (HD / 4), i = x % (HD / 4) * 4, rr = row0 + r;
+					if ((h.kind & 16) && !attn_len(a, h.s0 + rr / tg))
+						continue;              // (its own pieces say that it sees nothing)
+					float top = -INFINITY, sum = 0.0f, f[ATTN_WARPS];
+#pragma unroll
+					for (int w = 0; w < (int)ATTN_WARPS; w++)
+						top = fmaxf(top, s_m[w][r]);
+					const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+					for (int w = 0; w < (int)ATTN_WARPS; w++) {
+						f[w] = exp2_approx(s_m[w][r] - base);
+						sum += f[w] * s_l[w][r];
+					}
+					const size_t at = ((size_t)((h.s0 + rr / tg) * a.n_tok + rr % tg / a.gqa) * a.n_head +
+							   h.kvh * a.gqa + rr % a.gqa) * pieces;
+					const float inv = sum != 0.0f ? __fdiv_rn(1.0f, sum) : 0.0f;
+					if (i == 0) {
+						a.part_w[at + h.slot_at] = sum != 0.0f ? base + log2f(sum) : -INFINITY;
+						for (uint32_t j = 0; (h.kind & 32) && j < a.pre_splits; j++)
+							a.part_w[at + j] = -INFINITY;
+					}
+					float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+					for (int w = 0; w < (int)ATTN_WARPS; w++) {
+						const float4 p = *(const float4 *)(os + (w * ATTN_TILE_ROWS + r) * HD +
+										   (i ^ ((r & 3) * 8)));
+						v[0] += f[w] * p.x;
+						v[1] += f[w] * p.y;
+						v[2] += f[w] * p.z;
+						v[3] += f[w] * p.w;
+					}
+					*(float4 *)(a.part_o + (at + h.slot_at) * HD + i) =
+						make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+				}
+				fence_proxy_async_smem();
+				if (!together())                           // (s_m and s_l are free again)
+					break;
+			}
+			__syncwarp();
+			if (lane == 0)
+				mbar_arrive(&b_free[st]);
 		}
-		__syncwarp();
+		if (!ended && lane == 0)
+			*(volatile int *)a.err = ATTN_ERR_ROWS;
 	}
-	// join the warps: rows' maxima and sums, then the outputs through shared memory
-#pragma unroll
-	for (int h = 0; h < 2; h++) {
-		l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-		l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-		if (c == 0) {
-			s_m[warp][lane / 4 + 8 * h] = m[h];
-			s_l[warp][lane / 4 + 8 * h] = l[h];
-		}
-	}
-	__syncthreads();
-	float *os = reinterpret_cast<float *>(asm_);        // [warps][16][HD]
-#pragma unroll
-	for (int n = 0; n < NT; n++)
-#pragma unroll
-		for (int h = 0; h < 2; h++)
-			*(float2 *)(os + ((size_t)warp * ATTN_TILE_ROWS + lane / 4 + 8 * h) * HD + n * 8 +
-				    c * 2) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-	__syncthreads();
-	const uint32_t r = tid / 8, rr = tile * ATTN_TILE_ROWS + r;
-	if (rr >= n_rows)
-		return;
-	float top = -INFINITY, sum = 0.0f, f[ATTN_WARPS];
-#pragma unroll
-	for (int w = 0; w < (int)ATTN_WARPS; w++)
-		top = fmaxf(top, s_m[w][r]);
-	const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-	for (int w = 0; w < (int)ATTN_WARPS; w++) {
-		f[w] = exp2_approx(s_m[w][r] - base);
-		sum += f[w] * s_l[w][r];
-	}
-	const size_t at = ((size_t)((s0 + rr / tg) * a.n_tok + rr % tg / a.gqa) * a.n_head +
-			   kvh * a.gqa + rr % a.gqa) * pieces + slot_at;
-	const float inv = sum != 0.0f ? __fdiv_rn(1.0f, sum) : 0.0f;
-	if (tid % 8 == 0)
-		a.part_w[at] = sum != 0.0f ? base + log2f(sum) : -INFINITY;
-	for (uint32_t i = (tid % 8) * 4; i < HD; i += 32) {
-		float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-		for (int w = 0; w < (int)ATTN_WARPS; w++)
-#pragma unroll
-			for (int e = 0; e < 4; e++)
-				v[e] += f[w] * os[((size_t)w * ATTN_TILE_ROWS + r) * HD + i + e];
-		*(float4 *)(a.part_o + at * HD + i) =
-			make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-	}
+	if (a.beside)
+		pdl_wait();
 }
 
 // The pieces of each row joined: one warp a row (sequence, token, head).
@@ -543,37 +692,47 @@ attn_join_kernel(const __grid_constant__ AttnArgs a)
 	if (row >= (size_t)a.n_seq * a.n_tok * a.n_head)
 		return;
 	constexpr int EACH = HD / 32;
-	const uint32_t s = (uint32_t)(row / ((size_t)a.n_tok * a.n_head)), pieces = a.pre_splits + a.own_splits;
+	const uint32_t pieces = a.pre_splits + a.own_splits;
 	float v[EACH];
 #pragma unroll
 	for (int e = 0; e < EACH; e++)
 		v[e] = 0.0f;
-	if (attn_len(a, s) > 0) {
-		const uint32_t first = attn_group_of(a, s).keys ? 0 : a.pre_splits;
-		const float *w = a.part_w + row * pieces;
-		float top = -INFINITY, sum = 0.0f;
-		bool any = false;                       // (a NaN is no maximum, but it is a weight)
-		for (uint32_t j = first; j < pieces; j++) {
-			top = fmaxf(top, w[j]);
-			any |= w[j] != -INFINITY;
-		}
-		top = top == -INFINITY ? 0.0f : top;
-		if (any) {
-			for (uint32_t j = first; j < pieces; j++) {
-				if (w[j] == -INFINITY)
-					continue;
-				const float f = exp2_approx(w[j] - top);
-				sum += f;
-				const float *o = a.part_o + (row * pieces + j) * HD + lane * EACH;
+	// lane j has the weights of pieces j, j + 32, ...
+	constexpr int WORDS = ATTN_MAX_PIECES / 32;
+	const float *w = a.part_w + row * pieces;
+	float mine[WORDS], top = -INFINITY;
+	bool any = false;                               // (a NaN is no maximum, but it is a weight)
+#pragma unroll
+	for (int j = 0; j < WORDS; j++) {
+		mine[j] = lane + 32 * j < pieces ? w[lane + 32 * j] : -INFINITY;
+		top = fmaxf(top, mine[j]);
+		any |= mine[j] != -INFINITY;
+	}
+	for (int o = 16; o; o >>= 1)
+		top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+	top = top == -INFINITY ? 0.0f : top;
+	if (__any_sync(0xffffffffu, any)) {
+		float sum = 0.0f;
+#pragma unroll
+		for (int j = 0; j < WORDS; j++) {
+			const bool has = mine[j] != -INFINITY;
+			mine[j] = exp2_approx(mine[j] - top);
+			sum += mine[j];
+			for (uint32_t left = __ballot_sync(0xffffffffu, has); left; left &= left - 1) {
+				const int src = __ffs(left) - 1;
+				const float f = __shfl_sync(0xffffffffu, mine[j], src);
+				const float *o = a.part_o + (row * pieces + 32 * j + src) * HD + lane * EACH;
 #pragma unroll
 				for (int e = 0; e < EACH; e++)
 					v[e] += f * o[e];
 			}
-			const float inv = __fdiv_rn(1.0f, sum);
-#pragma unroll
-			for (int e = 0; e < EACH; e++)
-				v[e] *= inv;
 		}
+		for (int o = 16; o; o >>= 1)
+			sum += __shfl_xor_sync(0xffffffffu, sum, o);
+		const float inv = __fdiv_rn(1.0f, sum);
+#pragma unroll
+		for (int e = 0; e < EACH; e++)
+			v[e] *= inv;
 	}
 #pragma unroll
 	for (int e = 0; e < EACH; e += 2) {

@@ -27,8 +27,6 @@
 // piece is taken with the same maximum, so the result is the same.
 #pragma once
 
-#include <cuda.h>
-
 #include "attn.cuh"
 #include "tcgen05.cuh"
 
@@ -127,16 +125,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *u)
 		     : "memory");
 }
 
-// a box of (64 elements, positions of a page) of one head of one page
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, int x, int y, int z, int w,
-					    uint64_t *bar)
-{
-	asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-		     " [%0], [%1, {%2, %3, %4, %5}], [%6];"
-		     :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
-		     : "memory");
-}
-
 // codes of a wait that gave up, after the batched matvec's (5 to 13)
 constexpr int ATC_ERR_RING = 21, ATC_ERR_MMA = 22, ATC_ERR_ROWS = 23;
 
@@ -149,46 +137,13 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 	constexpr uint32_t COL_S = 0, COL_O = 256;      // S (and P) 128 columns a stream, then O
 	extern __shared__ uint8_t atc_raw[];
 	__shared__ __align__(8) uint64_t b_full[NB], b_free[NB], b_q, b_s[2], b_p[2], b_o[2], b_end;
-	__shared__ uint32_t s_tmem;
+	__shared__ uint32_t s_tmem, s_row[ATC_ROWS];
+	constexpr uint32_t NO_ROW = 0xffffffffu;
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 	const uint32_t q_at = (smem_addr(atc_raw) + 1023u) & ~1023u, ring = q_at + ATC_ROWS * HD * 2;
 	uint8_t *q_ptr = atc_raw + (q_at - smem_addr(atc_raw));
-	pdl_wait();
-	pdl_launch_dependents();
 
-	// which rows, which keys (every warp for itself)
-	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa, splits = a.pre_splits / 2;
-	uint32_t b = blockIdx.x;
-	const uint32_t u = b / (kvh_n * splits);
-	b -= u * kvh_n * splits;
-	const uint32_t piece = b / kvh_n, kvh = b - piece * kvh_n;
-	uint32_t g, tile;
-	if (!attn_find_unit(a, u, ATC_ROWS, &g, &tile))
-		return;
-	const AttnGroup gr = attn_group(a, g);
-	if (!gr.keys)
-		return;
-	int32_t k0 = 0, k1 = gr.keys;
-	attn_piece(k0, k1, piece, splits, ATC_KEYS);
-	const uint32_t n_rows = (gr.s1 - gr.s0) * tg, row0 = tile * ATC_ROWS;
-	const bool halves = n_rows - row0 > 128;
-	const uint32_t tiles = (uint32_t)(k1 - k0 + (int32_t)ATC_KEYS - 1) / ATC_KEYS;
-	const uint32_t pieces = a.pre_splits + a.own_splits;
-	// row r of the unit: its place in q, and in the pieces
-	auto row_of = [&](uint32_t r) {
-		const uint32_t s = gr.s0 + r / tg, x = r % tg;
-		return (size_t)(s * a.n_tok + x / a.gqa) * a.n_head + kvh * a.gqa + x % a.gqa;
-	};
-	if (!tiles) {
-		for (uint32_t r = row0 + threadIdx.x; r < min(row0 + ATC_ROWS, n_rows); r += ATC_THREADS) {
-			a.part_w[row_of(r) * pieces + 2 * piece] = -INFINITY;
-			a.part_w[row_of(r) * pieces + 2 * piece + 1] = -INFINITY;
-		}
-		return;
-	}
-	// the tiles of stream i
-	auto count = [&](uint32_t i) { return halves ? tiles : (tiles + 1 - i) / 2; };
-
+	// barriers and tensor memory while the kernel before is still running
 	if (warp == 8) {
 		if (lane == 0) {
 			for (uint32_t i = 0; i < NB; i++) {
@@ -208,26 +163,63 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 		tmem_alloc(&s_tmem, 512);
 		tmem_relinquish();
 	}
+	pdl_wait();
+	pdl_launch_dependents();
+
+	// which rows, which keys (every warp for itself)
+	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa, splits = a.pre_splits / 2;
+	uint32_t b = blockIdx.x;
+	const uint32_t u = b / (kvh_n * splits);
+	b -= u * kvh_n * splits;
+	const uint32_t piece = b / kvh_n, kvh = b - piece * kvh_n;
+	uint32_t g = 0, tile = 0;
+	AttnGroup gr = {0, 0, 0, -1};
+	if (attn_find_unit(a, u, ATC_ROWS, &g, &tile))
+		gr = attn_group(a, g);
+	int32_t k0 = 0, k1 = gr.keys;
+	attn_piece(k0, k1, piece, splits, ATC_KEYS);
+	const uint32_t n_rows = (gr.s1 - gr.s0) * tg, row0 = tile * ATC_ROWS;
+	const bool halves = n_rows - row0 > 128;
+	const uint32_t tiles = (uint32_t)(k1 - k0 + (int32_t)ATC_KEYS - 1) / ATC_KEYS;
+	const uint32_t pieces = a.pre_splits + a.own_splits;
+	// a row of the unit by its number among q's rows: (sequence, token, head)
+	if (threadIdx.x < ATC_ROWS) {
+		// (none: behind the last, or a query that sees nothing, as its own pieces say)
+		const uint32_t r = row0 + threadIdx.x, s = gr.s0 + r / tg, x = r % tg;
+		s_row[threadIdx.x] = r < n_rows && attn_len(a, s)
+					     ? (s * a.n_tok + x / a.gqa) * a.n_head + kvh * a.gqa + x % a.gqa
+					     : NO_ROW;
+	}
+	// the tiles of stream i
+	auto count = [&](uint32_t i) { return halves ? tiles : (tiles + 1 - i) / 2; };
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
 	const uint32_t tmem = s_tmem;
 
-	if (warp == 9) {
+	if (!tiles) {
+		// nothing in this piece (a group with fewer rows or keys than the launch has room for)
+		if (gr.keys && threadIdx.x < ATC_ROWS && s_row[threadIdx.x] != NO_ROW) {
+			float *w = a.part_w + (size_t)s_row[threadIdx.x] * pieces + 2 * piece;
+			w[0] = w[1] = -INFINITY;
+		}
+	} else if (warp == 9) {
 		// ---- K and V tiles into the ring: K of tile j is copy 2 j, V copy 2 j + 1
-		const uint32_t per = ATC_KEYS / a.p.page;        // pages a tile
-		const int32_t *row = a.p.table + (size_t)gr.slot * a.p.max_pages + k0 / (int32_t)a.p.page;
-		const uint32_t left = (uint32_t)(k1 - k0) / a.p.page;      // pages of the piece
-		const uint32_t my_page = lane % per, my_slab = lane / per;
+		const uint32_t box = min(a.p.page, 64u), per = ATC_KEYS / box;     // positions; boxes a tile
+		const int32_t *row = a.p.table + (size_t)gr.slot * a.p.max_pages;
+		const uint32_t my_box = lane % per, my_slab = lane / per;
 		bool ok = true;
 		uint32_t c = 0;
-		for (uint32_t j = 0; j < tiles && ok; j++) {
-			// a page past the piece, or no page at all, reads as zeros
-			int32_t page = (int32_t)a.p.n_pages;
-			if (j * per + my_page < left) {
-				page = __ldcg(&row[j * per + my_page]);
-				page = (uint32_t)page < a.p.n_pages ? page : (int32_t)a.p.n_pages;
-			}
+		// a page past the piece, or no page at all, reads as zeros
+		auto pos_of = [&](uint32_t j) { return (uint32_t)k0 + j * ATC_KEYS + my_box * box; };
+		auto page_of = [&](uint32_t j) {
+			const uint32_t pos = pos_of(j);
+			const uint32_t page = pos < (uint32_t)k1 ? (uint32_t)__ldcg(&row[pos / a.p.page]) : a.p.n_pages;
+			return (int)min(page, a.p.n_pages);
+		};
+		int page = page_of(0), next = 0;
+		for (uint32_t j = 0; j < tiles && ok; j++, page = next) {
+			next = page_of(j + 1);
 			for (int v = 0; v < 2; v++, c++) {
 				const uint32_t at = c % NB;
 				if (c >= NB)
@@ -239,9 +231,9 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 					mbar_arrive_expect_tx(&b_full[at], TILE);
 				__syncwarp();
 				if (my_slab < SLABS)
-					tma_load_4d(ring + at * TILE + my_slab * ATC_SLAB + my_page * a.p.page * 128,
-						    v ? &vmap : &kmap, (int)(my_slab * 64), 0, (int)kvh, page,
-						    &b_full[at]);
+					tma_load_4d(ring + at * TILE + my_slab * ATC_SLAB + my_box * box * 128,
+						    v ? &vmap : &kmap, (int)(my_slab * 64),
+						    (int)(pos_of(j) % a.p.page), (int)kvh, page, &b_full[at]);
 				__syncwarp();
 			}
 		}
@@ -314,16 +306,22 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 		// ---- rows: Q into shared memory first (swizzled as the tensor copies would)
 		const uint32_t rows = halves ? 256 : 128;
 		const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;     // scale > 0 from here on
-		for (uint32_t x = threadIdx.x; x < rows * (HD / 8); x += 256) {
-			const uint32_t r = x / (HD / 8), w = x % (HD / 8);
-			uint4 v = make_uint4(0, 0, 0, 0);
-			if (row0 + r < n_rows)
-				v = *(const uint4 *)((const T *)a.q + row_of(row0 + r) * HD + w * 8);
-			v.x ^= flip;
-			v.y ^= flip;
-			v.z ^= flip;
-			v.w ^= flip;
-			*(uint4 *)(q_ptr + (w / 8) * (ATC_ROWS * 128) + r * 128 + (((w % 8) ^ (r & 7)) << 4)) = v;
+		constexpr uint32_t QW = HD / 8, EACH = 128 * QW / 256;      // words a row; a thread's in 128 rows
+		const uint32_t w = threadIdx.x % QW;
+		for (uint32_t r0 = 0; r0 < rows; r0 += 128) {
+			uint4 v[EACH];
+#pragma unroll
+			for (uint32_t e = 0; e < EACH; e++) {
+				const uint32_t row = s_row[r0 + e * (256 / QW) + threadIdx.x / QW];
+				v[e] = row == NO_ROW ? make_uint4(0, 0, 0, 0)
+						     : __ldcg((const uint4 *)((const T *)a.q + (size_t)row * HD + w * 8));
+			}
+#pragma unroll
+			for (uint32_t e = 0; e < EACH; e++) {
+				const uint32_t r = r0 + e * (256 / QW) + threadIdx.x / QW;
+				*(uint4 *)(q_ptr + (w / 8) * (ATC_ROWS * 128) + r * 128 + (((w % 8) ^ (r & 7)) << 4)) =
+					make_uint4(v[e].x ^ flip, v[e].y ^ flip, v[e].z ^ flip, v[e].w ^ flip);
+			}
 		}
 		fence_proxy_async_smem();
 		mbar_arrive(&b_q);
@@ -402,35 +400,41 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 			tc_fence_before();
 			mbar_arrive(&b_p[i]);
 		}
-		if (ok && mine)
-			ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_o[i], (mine - 1) & 1, WAIT_LIMIT_NS));
+		// all MMAs are done: the outputs go out through the ring, 32 columns of a warp's 32
+		// rows at a time, so that a row's 128 bytes leave together
+		ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(&b_end, 0, WAIT_LIMIT_NS));
 		if (!ok && lane == 0)
 			*(volatile int *)a.err = ATC_ERR_ROWS;
 		if (ok) {
 			tc_fence_after();
-			const uint32_t r = row0 + (halves ? i * 128 : 0) + quarter * 32 + lane;
-			const bool real = r < n_rows;
-			const size_t at = real ? row_of(r) * pieces + 2 * piece + (halves ? 0 : i) : 0;
+			const uint32_t r = (halves ? i * 128 : 0) + quarter * 32, my = s_row[r + lane];
+			const uint32_t col = 2 * piece + (halves ? 0 : i);
 			const float inv = l != 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
-			if (real) {
-				a.part_w[at] = l != 0.0f ? (m == -INFINITY ? 0.0f : m * scale) + log2f(l) : -INFINITY;
+			if (my != NO_ROW) {
+				float *w = a.part_w + (size_t)my * pieces + col;
+				w[0] = l != 0.0f ? (m == -INFINITY ? 0.0f : m * scale) + log2f(l) : -INFINITY;
 				if (halves)
-					a.part_w[at + 1] = -INFINITY;
+					w[1] = -INFINITY;
 			}
-			if (mine) {
-#pragma unroll 1
-				for (int c = 0; c < HD / 32; c++) {
-					float o[32];
-					tmem_ld32(to + 32 * c, o);
-					tmem_wait_ld();
-					tmem_loaded32(o);
-					if (real)
+			float *stage = reinterpret_cast<float *>(q_ptr + ATC_ROWS * HD * 2) + warp * (32 * 36);
+			for (int c = 0; mine && c < HD / 32; c++) {
+				float o[32];
+				tmem_ld32(to + 32 * c, o);
+				tmem_wait_ld();
+				tmem_loaded32(o);
 #pragma unroll
-						for (int e = 0; e < 32; e += 4)
-							*(float4 *)(a.part_o + at * HD + 32 * c + e) =
-								make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv,
-									    o[e + 3] * inv);
+				for (int e = 0; e < 32; e += 4)
+					*(float4 *)(stage + lane * 36 + e) = make_float4(o[e] * inv, o[e + 1] * inv,
+											 o[e + 2] * inv, o[e + 3] * inv);
+				__syncwarp();
+#pragma unroll
+				for (int e = 0; e < 8; e++) {
+					const uint32_t row = e * 4 + lane / 8, at = s_row[r + row];
+					if (at != NO_ROW)
+						*(float4 *)(a.part_o + ((size_t)at * pieces + col) * HD + 32 * c +
+							    (lane % 8) * 4) = *(float4 *)(stage + row * 36 + (lane % 8) * 4);
 				}
+				__syncwarp();
 			}
 		}
 		tc_fence_before();

@@ -171,14 +171,15 @@ const char *attention_fault(const charsiu_gpu_pages *p, const charsiu_gpu_attent
 		return "the batch lacks an array";
 	if (!a->n_tok || !a->n_head || a->n_head % p->n_head_kv)
 		return "n_tok is 0, or n_head no multiple of n_head_kv";
-	if ((uint64_t)a->n_seq * a->n_tok * a->n_head > 0x7fffffffull || a->n_group > a->n_seq)
+	if ((uint64_t)a->n_seq * a->n_tok * a->n_head > (1ull << 25) || a->n_group > a->n_seq)
 		return "the batch is larger than the call takes";
 	if (a->out_type != TYPE_F32 && a->out_type != p->type)
 		return "out_type is neither fp32 nor the cache's type";
 	return "";
 }
 
-constexpr uint32_t ATTN_CTAS_PER_SM = 3, ATTN_MAX_SPLITS = 32;
+constexpr uint32_t ATTN_CTAS_PER_SM = 2;     // of the rows kernel, by its shared memory
+constexpr uint32_t ATTN_LONG = 2048;         // keys: about the most in a piece of a sequence
 
 // How the work is cut. Returns whether the prefixes go to the tensor cores.
 bool attention_plan(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gpu_attention *b,
@@ -196,7 +197,11 @@ bool attention_plan(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gp
 	a->own_tiles = (rows + ATTN_TILE_ROWS - 1) / ATTN_TILE_ROWS;
 	a->own_splits = splits((uint64_t)b->n_seq * a->own_tiles * p->n_head_kv, ATTN_CTAS_PER_SM * sms,
 			       b->max_len / ATTN_GRAIN + 1);
-	a->pre_units = a->pre_splits = 0;
+	// in a large batch a long sequence is cut all the same, or it would be the last to end
+	a->own_grain = a->own_splits > 1 ? ATTN_GRAIN : 4 * ATTN_GRAIN;
+	const uint32_t by_length = b->max_len / ATTN_LONG < ATTN_MAX_SPLITS ? b->max_len / ATTN_LONG : ATTN_MAX_SPLITS;
+	a->own_splits = a->own_splits > by_length ? a->own_splits : by_length;
+	a->pre_units = a->pre_splits = a->rows_splits = 0;
 	if (!b->n_group)
 		return false;
 	const bool tc = all >= 32;
@@ -205,6 +210,7 @@ bool attention_plan(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gp
 	a->pre_splits = tc ? 2 * splits((uint64_t)a->pre_units * p->n_head_kv, sms, b->max_len / ATC_KEYS + 1)
 			   : splits((uint64_t)a->pre_units * p->n_head_kv, ATTN_CTAS_PER_SM * sms,
 				    b->max_len / ATTN_GRAIN + 1);
+	a->rows_splits = tc ? 0 : a->pre_splits;
 	a->pre_units += b->n_group;          // each group may end in a part of a unit
 	return tc;
 }
@@ -219,6 +225,8 @@ size_t attention_bytes(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu
 	const uint64_t sms = (uint64_t)layer_sms(g);
 	uint64_t parts = n + ATTN_CTAS_PER_SM * sms / (tiles * kv) + 1;
 	parts = parts < most ? parts : most;
+	const uint64_t by_length = n * (b->max_len / ATTN_LONG);
+	parts = parts > by_length ? parts : by_length < most ? by_length : most;
 	if (b->n_group) {
 		const uint64_t pre = 2 * (n + sms * ATC_ROWS / (rows * kv) + 1);
 		parts += pre < 2 * most ? pre : 2 * most;
@@ -226,8 +234,8 @@ size_t attention_bytes(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu
 	return (size_t)(parts * b->n_tok * b->n_head * (p->head_dim + 1) * sizeof(float) + 15) / 16 * 16;
 }
 
-// K or V of one layer as (element, position, head, page); boxes of 64 elements and a
-// page's positions. A dimension of one element has no stride to speak of.
+// K or V of one layer as (element, position, head, page); boxes of 64 elements and at
+// most 64 positions of a page. A dimension of one element has no stride to speak of.
 bool attention_map(CUtensorMap *map, const charsiu_gpu_pages *p, const void *base, unsigned layer)
 {
 	const auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encode());
@@ -237,7 +245,7 @@ bool attention_map(CUtensorMap *map, const charsiu_gpu_pages *p, const void *bas
 	const cuuint64_t row = 2ull * p->head_dim;
 	const cuuint64_t strides[3] = {2 * p->pos_stride, p->n_head_kv > 1 ? 2 * p->head_stride : row,
 				       p->n_pages > 1 ? 2 * p->page_stride : row};
-	const cuuint32_t box[4] = {64, p->page, 1, 1}, ones[4] = {1, 1, 1, 1};
+	const cuuint32_t box[4] = {64, p->page < 64 ? p->page : 64, 1, 1}, ones[4] = {1, 1, 1, 1};
 	return enc(map, p->type == TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
 		   4, (uint8_t *)const_cast<void *>(base) + 2 * layer * p->layer_stride, dims, strides, box, ones,
 		   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -248,26 +256,26 @@ template <typename T, int HD>
 int attention(charsiu_gpu *g, AttnArgs &a, bool tc, void *stream)
 {
 	static uint64_t smem_done, tc_done;
-	if (!allow_smem(g, attn_rows_kernel<T, HD>, attn_rows_smem<HD>(), smem_done))
+	CUtensorMap kmap, vmap;
+	if (!attention_map(&kmap, &a.p, a.p.k, a.layer) || !attention_map(&vmap, &a.p, a.p.v, a.layer))
+		return refuse(g, "the cache's strides cannot be described to the copy engine");
+	if (!allow_smem(g, attn_rows_kernel<T, HD>, AttnRing<HD>::SMEM, smem_done) ||
+	    !allow_smem(g, attn_tc_kernel<T, HD>, atc_smem<HD>(), tc_done))
 		return -1;
-	const uint64_t pre = (uint64_t)a.p.n_head_kv * a.pre_units * (tc ? a.pre_splits / 2 : a.pre_splits);
-	const uint64_t own = (uint64_t)a.p.n_head_kv * a.n_seq * a.own_tiles * a.own_splits;
-	if (pre + own > 0x7fffffffull)
-		return refuse(g, "the batch is larger than the call takes");
 	if (tc) {
-		CUtensorMap kmap, vmap;
-		if (!attention_map(&kmap, &a.p, a.p.k, a.layer) || !attention_map(&vmap, &a.p, a.p.v, a.layer))
-			return refuse(g, "the cache's strides cannot be described to the copy engine");
-		if (!allow_smem(g, attn_tc_kernel<T, HD>, atc_smem<HD>(), tc_done) ||
-		    !launch(g, stream, attn_tc_kernel<T, HD>, dim3((unsigned)pre), ATC_THREADS, atc_smem<HD>(), a,
+		if (!launch(g, stream, attn_tc_kernel<T, HD>,
+			    dim3(a.pre_units * a.p.n_head_kv * (a.pre_splits / 2)), ATC_THREADS, atc_smem<HD>(), a,
 			    kmap, vmap))
 			return -1;
-		a.pre_units = 0;
 		a.beside = 1;
+		a.pre_units = 0;
 	}
+	const uint64_t items = (uint64_t)a.p.n_head_kv * ((uint64_t)a.pre_units * a.rows_splits +
+							  (uint64_t)a.n_seq * a.own_tiles * a.own_splits);
+	const uint64_t grid = ATTN_CTAS_PER_SM * (uint64_t)layer_sms(g);
 	const uint64_t rows = (uint64_t)a.n_seq * a.n_tok * a.n_head;
-	return launch(g, stream, attn_rows_kernel<T, HD>, dim3((unsigned)(own + (tc ? 0 : pre))),
-		      ATTN_WARPS * 32, attn_rows_smem<HD>(), a) &&
+	return launch(g, stream, attn_rows_kernel<T, HD>, dim3((unsigned)(items < grid ? items : grid)),
+		      ATTN_THREADS, AttnRing<HD>::SMEM, a, kmap, vmap) &&
 			       launch(g, stream, attn_join_kernel<T, HD>,
 				      dim3((unsigned)((rows + 7) / 8)), 256, 0, a)
 		       ? 0
