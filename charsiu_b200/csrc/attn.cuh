@@ -52,14 +52,19 @@ struct AttnArgs {
 // (Lengths, tables and queries are read past L1: the rows kernel may start without
 // a wait of its own, see there.)
 
-// the length of sequence s of the batch; 0 for a padded one
-__device__ __forceinline__ int32_t attn_len(const AttnArgs &a, uint32_t s)
+// the length of a slot; 0 for none
+__device__ __forceinline__ int32_t attn_slot_len(const AttnArgs &a, int32_t slot)
 {
-	const int32_t slot = __ldcg(&a.slots[s]);
 	if (!pages_slot_ok(a.p, slot))
 		return 0;
 	const int64_t len = __ldcg(&a.p.len[slot]), most = (int64_t)a.p.max_pages * a.p.page;
 	return (int32_t)(len < 0 ? 0 : len > most ? most : len);
+}
+
+// the length of sequence s of the batch; 0 for a padded one
+__device__ __forceinline__ int32_t attn_len(const AttnArgs &a, uint32_t s)
+{
+	return attn_slot_len(a, __ldcg(&a.slots[s]));
 }
 
 // What the queries of a group share: sequences [s0, s1), their `keys` first keys
@@ -69,32 +74,38 @@ struct AttnGroup {
 	int32_t keys, slot;
 };
 
-// by a whole warp
-__device__ __forceinline__ AttnGroup attn_group(const AttnArgs &a, uint32_t g)
+// of the group with these bounds and told shared pages; by a whole warp
+__device__ __forceinline__ AttnGroup attn_group(const AttnArgs &a, int32_t b0, int32_t b1, int32_t told)
 {
 	AttnGroup r;
-	const int32_t b0 = __ldcg(&a.group[g]), b1 = __ldcg(&a.group[g + 1]);
 	r.s0 = b0 < 0 ? 0 : b0 > (int32_t)a.n_seq ? a.n_seq : (uint32_t)b0;
 	r.s1 = b1 < (int32_t)r.s0 ? r.s0 : b1 > (int32_t)a.n_seq ? a.n_seq : (uint32_t)b1;
-	int32_t least = 0x7fffffff;
+	int32_t least = 0x7fffffff, mine = -1;
 	uint32_t first = 0xffffffffu;
-	for (uint32_t s = r.s0 + (threadIdx.x & 31); s < r.s1; s += 32) {
-		const int32_t len = attn_len(a, s);
-		if (len > 0) {
-			least = min(least, len - (int32_t)a.n_tok + 1);
-			first = min(first, s);
-		}
+	for (uint32_t s = r.s0 + (threadIdx.x & 31); s < r.s1; s += 64) {
+		// two at a time: their slots, then their lengths
+		const int32_t sl[2] = {__ldcg(&a.slots[s]), s + 32 < r.s1 ? __ldcg(&a.slots[s + 32]) : -1};
+		const int32_t len[2] = {attn_slot_len(a, sl[0]), attn_slot_len(a, sl[1])};
+#pragma unroll
+		for (int j = 0; j < 2; j++)
+			if (len[j] > 0) {
+				least = min(least, len[j] - (int32_t)a.n_tok + 1);
+				if (s + 32 * j < first) {
+					first = s + 32 * j;
+					mine = sl[j];
+				}
+			}
 	}
 	least = __reduce_min_sync(0xffffffffu, least);
-	first = __reduce_min_sync(0xffffffffu, first);
+	const uint32_t lowest = __reduce_min_sync(0xffffffffu, first);
+	const uint32_t who = __ballot_sync(0xffffffffu, first == lowest && mine >= 0);
 	r.keys = 0;
 	r.slot = -1;
-	if (first != 0xffffffffu && least > 0) {
-		int32_t pages = __ldcg(&a.shared[g]);
-		pages = min(pages, (int32_t)a.p.max_pages);
+	if (who && least > 0) {
+		int32_t pages = min(told, (int32_t)a.p.max_pages);
 		pages = min(pages, least / (int32_t)a.p.page);
 		r.keys = pages > 0 ? pages * (int32_t)a.p.page : 0;
-		r.slot = __ldcg(&a.slots[first]);
+		r.slot = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
 	}
 	return r;
 }
@@ -104,11 +115,15 @@ __device__ __forceinline__ AttnGroup attn_group_of(const AttnArgs &a, uint32_t s
 {
 	for (uint32_t g0 = 0; g0 < a.n_group; g0 += 32) {
 		const uint32_t g = g0 + (threadIdx.x & 31);
-		const bool in = g < a.n_group && __ldcg(&a.group[g]) <= (int32_t)s &&
-				(int32_t)s < __ldcg(&a.group[g + 1]);
-		const uint32_t who = __ballot_sync(0xffffffffu, in);
-		if (who)
-			return attn_group(a, g0 + __ffs(who) - 1);
+		const bool real = g < a.n_group;
+		const int32_t b0 = real ? __ldcg(&a.group[g]) : 0, b1 = real ? __ldcg(&a.group[g + 1]) : 0;
+		const int32_t told = real ? __ldcg(&a.shared[g]) : 0;
+		const uint32_t who = __ballot_sync(0xffffffffu, b0 <= (int32_t)s && (int32_t)s < b1);
+		if (who) {
+			const int src = __ffs(who) - 1;
+			return attn_group(a, __shfl_sync(0xffffffffu, b0, src), __shfl_sync(0xffffffffu, b1, src),
+					  __shfl_sync(0xffffffffu, told, src));
+		}
 	}
 	AttnGroup r;
 	r.s0 = r.s1 = s;
@@ -120,18 +135,17 @@ __device__ __forceinline__ AttnGroup attn_group_of(const AttnArgs &a, uint32_t s
 // Unit u of all groups' row tiles (`rows` rows each): its group and the tile in
 // it; false past the last. By a whole warp.
 __device__ __forceinline__ bool attn_find_unit(const AttnArgs &a, uint32_t u, uint32_t rows,
-					       uint32_t *g, uint32_t *tile)
+					       AttnGroup *g, uint32_t *tile)
 {
 	const uint32_t lane = threadIdx.x & 31;
 	uint32_t before = 0;
 	for (uint32_t g0 = 0; g0 < a.n_group; g0 += 32) {
-		uint32_t n = 0;
-		if (g0 + lane < a.n_group) {
-			const int32_t b0 = max(__ldcg(&a.group[g0 + lane]), 0);
-			const int32_t b1 = min(__ldcg(&a.group[g0 + lane + 1]), (int32_t)a.n_seq);
-			if (b1 > b0)
-				n = ((uint32_t)(b1 - b0) * a.n_tok * a.gqa + rows - 1) / rows;
-		}
+		const bool real = g0 + lane < a.n_group;
+		const int32_t b0 = real ? __ldcg(&a.group[g0 + lane]) : 0;
+		const int32_t b1 = real ? __ldcg(&a.group[g0 + lane + 1]) : 0;
+		const int32_t told = real ? __ldcg(&a.shared[g0 + lane]) : 0;
+		const int32_t c0 = max(b0, 0), c1 = min(b1, (int32_t)a.n_seq);
+		const uint32_t n = c1 > c0 ? ((uint32_t)(c1 - c0) * a.n_tok * a.gqa + rows - 1) / rows : 0;
 		uint32_t inc = n;
 		for (int o = 1; o < 32; o <<= 1) {
 			const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
@@ -142,8 +156,9 @@ __device__ __forceinline__ bool attn_find_unit(const AttnArgs &a, uint32_t u, ui
 		const uint32_t who = __ballot_sync(0xffffffffu, u >= lo && u < lo + n);
 		if (who) {
 			const int src = __ffs(who) - 1;
-			*g = g0 + src;
 			*tile = u - __shfl_sync(0xffffffffu, lo, src);
+			*g = attn_group(a, __shfl_sync(0xffffffffu, b0, src), __shfl_sync(0xffffffffu, b1, src),
+					__shfl_sync(0xffffffffu, told, src));
 			return true;
 		}
 		before += __shfl_sync(0xffffffffu, inc, 31);
@@ -246,8 +261,7 @@ struct AttnRing {
 };
 
 struct AttnStage {
-	uint32_t kind;        // 1: an item's first stage, 2: its last, 4: no keys at all, 8: the end,
-			      // 16: of a prefix, 32: its rows have no prefix
+	uint32_t kind;        // 1: an item's first stage, 2: its last, 8: the end, 16: of a prefix
 	uint32_t s0, n_rows, tile, kvh, slot_at;
 	int32_t key0, k1;     // the stage's first key; the piece's end
 	int32_t len;          // the sequence's length (a prefix is seen whole)
@@ -315,12 +329,8 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 						mbar_wait_bounded(&b_free[st], (c / NS - 1) & 1, WAIT_LIMIT_NS));
 			if (!ok)
 				return;
-			uint32_t boxes = 0;
-			if (!(h.kind & 4)) {
-				const uint32_t keys = min((uint32_t)(h.k1 - h.key0), R::KEYS);
-				boxes = (keys + box - 1) / box;
-			}
-			const uint32_t q_rows = (h.kind & 5) == 1 ? min(h.n_rows - h.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS) : 0;
+			const uint32_t keys = min((uint32_t)(h.k1 - h.key0), R::KEYS), boxes = (keys + box - 1) / box;
+			const uint32_t q_rows = h.kind & 1 ? min(h.n_rows - h.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS) : 0;
 			// this lane's box: which positions, which 64 elements; K and V alike
 			const uint32_t mine = lane % (R::KEYS / 16), slab = lane / (R::KEYS / 16);
 			const uint32_t pos = (uint32_t)h.key0 + mine * box;
@@ -360,10 +370,8 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 				b -= u * kvh_n * a.rows_splits;
 				const uint32_t piece = b / kvh_n;
 				h.kvh = b - piece * kvh_n;
-				uint32_t g;
-				if (!attn_find_unit(a, u, ATTN_TILE_ROWS, &g, &h.tile))
-					continue;
-				gr = attn_group(a, g);
+				if (!attn_find_unit(a, u, ATTN_TILE_ROWS, &gr, &h.tile))
+					continue;                      // (past the last)
 				if (!gr.keys)
 					continue;
 				h.s0 = gr.s0;
@@ -394,22 +402,29 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 				attn_piece(k0, h.k1, piece, a.own_splits, a.own_grain);
 				h.slot_at = a.pre_splits + piece;
 			}
-			if (k0 >= h.k1) {
-				h.kind = kind | 7;
-				h.key0 = k0;
-				push(h, nullptr);
-				continue;
+			const uint32_t rows = min(h.n_rows - h.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS);
+			if (lane < rows && (k0 >= h.k1 || (kind & 32))) {
+				// no keys, or no prefix: the weights say so
+				const uint32_t r = h.tile * ATTN_TILE_ROWS + lane, s = h.s0 + r / tg, x = r % tg;
+				float *w = a.part_w + ((size_t)(s * a.n_tok + x / a.gqa) * a.n_head + h.kvh * a.gqa +
+						       x % a.gqa) * pieces;
+				if (k0 >= h.k1 && (!(kind & 16) || attn_len(a, s)))
+					w[h.slot_at] = -INFINITY;
+				for (uint32_t j = 0; (kind & 32) && j < a.pre_splits; j++)
+					w[j] = -INFINITY;
 			}
+			if (k0 >= h.k1)
+				continue;
 			const int32_t *row = a.p.table + (size_t)slot * a.p.max_pages;
 			for (int32_t key0 = k0; key0 < h.k1 && ok; key0 += (int32_t)R::KEYS) {
-				h.kind = kind | (key0 == k0 ? 1u : 0u) | (key0 + (int32_t)R::KEYS >= h.k1 ? 2u : 0u);
+				h.kind = (kind & 16) | (key0 == k0 ? 1u : 0u) | (key0 + (int32_t)R::KEYS >= h.k1 ? 2u : 0u);
 				h.key0 = key0;
 				push(h, row);
 			}
 		}
 		// the end; then every copy issued lands before the CTA leaves
 		AttnStage end = {};
-		end.kind = 8 | 4;
+		end.kind = 8;
 		if (ok)
 			push(end, nullptr);
 		if (!ok && lane == 0)
@@ -446,8 +461,6 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 #pragma unroll
 				for (int n = 0; n < NT; n++)
 					o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-			}
-			if ((h.kind & 5) == 1) {
 				// this thread's rows of the accumulators: lane / 4 and 8 more
 #pragma unroll
 				for (int e = 0; e < 2; e++) {
@@ -471,7 +484,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 			}
 			const uint32_t ks_ = ring + st * R::STAGE, vs = ks_ + R::HALF, w0 = warp * R::WKEYS;
 			const int32_t key0 = h.key0 + (int32_t)w0;
-			if (!(h.kind & 4) && key0 < h.k1) {
+			if (key0 < h.k1) {
 				constexpr int NK = R::WKEYS / 8;
 				float s[NK][4];
 #pragma unroll
@@ -647,11 +660,8 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 					const size_t at = ((size_t)((h.s0 + rr / tg) * a.n_tok + rr % tg / a.gqa) * a.n_head +
 							   h.kvh * a.gqa + rr % a.gqa) * pieces;
 					const float inv = sum != 0.0f ? __fdiv_rn(1.0f, sum) : 0.0f;
-					if (i == 0) {
+					if (i == 0)
 						a.part_w[at + h.slot_at] = sum != 0.0f ? base + log2f(sum) : -INFINITY;
-						for (uint32_t j = 0; (h.kind & 32) && j < a.pre_splits; j++)
-							a.part_w[at + j] = -INFINITY;
-					}
 					float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
 					for (int w = 0; w < (int)ATTN_WARPS; w++) {
@@ -718,13 +728,23 @@ attn_join_kernel(const __grid_constant__ AttnArgs a)
 			const bool has = mine[j] != -INFINITY;
 			mine[j] = exp2_approx(mine[j] - top);
 			sum += mine[j];
-			for (uint32_t left = __ballot_sync(0xffffffffu, has); left; left &= left - 1) {
-				const int src = __ffs(left) - 1;
-				const float f = __shfl_sync(0xffffffffu, mine[j], src);
-				const float *o = a.part_o + (row * pieces + 32 * j + src) * HD + lane * EACH;
+			for (uint32_t left = __ballot_sync(0xffffffffu, has); left;) {
+				float f[4], p[4][EACH];          // four pieces' outputs on their way at a time
 #pragma unroll
-				for (int e = 0; e < EACH; e++)
-					v[e] += f * o[e];
+				for (int k = 0; k < 4; k++, left &= left - 1) {
+					const int src = left ? __ffs(left) - 1 : 0;
+					f[k] = __shfl_sync(0xffffffffu, mine[j], src);
+					const float *o = a.part_o + (row * pieces + 32 * j + src) * HD + lane * EACH;
+#pragma unroll
+					for (int e = 0; e < EACH; e++)
+						p[k][e] = left ? o[e] : 0.0f;
+					f[k] = left ? f[k] : 0.0f;
+				}
+#pragma unroll
+				for (int k = 0; k < 4; k++)
+#pragma unroll
+					for (int e = 0; e < EACH; e++)
+						v[e] += f[k] * p[k][e];
 			}
 		}
 		for (int o = 16; o; o >>= 1)

@@ -10,17 +10,23 @@
 //
 //   warp 9      copies K and V tiles of 128 keys, page by page, by tensor copies
 //               (128-byte swizzle) into a ring
-//   warp 8      issues the MMAs: S = Q K^T (M = 128 rows, N = 128 keys) into tensor
-//               memory, and O += P V with P read from tensor memory, where
-//               it lies over the S it was made of, and V as an operand whose N
-//               (hd) is the contiguous side
+//   warp 8      issues the MMAs, in steps of 64 keys (half a tile): S = Q K^T (M = 128
+//               rows, N = 64 keys) into tensor memory, and O += P V with P read
+//               from tensor memory, where it lies over the S it was made of, and V
+//               as an operand whose N (hd) is the contiguous side
 //   warps 0-7   two streams of 128 rows, a thread a row: scores out of tensor
 //               memory, maximum, exponentials, the sum, P back
 //
-// While one stream is in its exponentials the tensor cores work for the other. With
-// more than 128 rows in the unit the streams are its two halves; with fewer they
-// are the same rows over the even and the odd tiles of keys, joined with the other
-// pieces at the end.
+// A stream's scores have two buffers and run two steps ahead of its outputs, so the
+// exponentials of a step find their scores ready, and the tensor cores work for
+// one stream while the other is in its exponentials. With more than 128 rows in the
+// unit the streams are its two halves; with fewer they are the same rows over the
+// even and the odd tiles, joined with the other pieces at the end.
+//
+// The MMA thread must do next to nothing between MMAs: one takes 64 cycles (N = 128, at
+// the tensor cores' full rate; 48 for scores of N = 64, by the shared memory they read),
+// and descriptors put together in 64 bits for each cost 120 to 170. Here a descriptor's
+// high word is a constant and its low word a running sum.
 //
 // O is scaled only where a row's maximum has grown by more than 2^8 since it was
 // last taken (P stays below 2^8, exact enough in both types); the weight of the
@@ -33,10 +39,13 @@
 namespace cgpu {
 
 constexpr uint32_t ATC_KEYS = 128, ATC_ROWS = 256;
+constexpr uint32_t ATC_STEP = 64;                    // keys of a step: half a tile
 constexpr int ATC_THREADS = 320;
 constexpr uint32_t ATC_SLAB = ATC_KEYS * 128;        // 128 rows of 64 elements
 
-// Tiles in the ring: what fits beside Q
+// Tiles in the ring: what fits beside Q; one more where Q is 128 rows (a half of it is a
+// tile). Streams on the same rows need it: scores run two steps ahead of outputs, so
+// the second stream asks for K of tile 3 while V of tile 0 is still to be used.
 template <int HD>
 __host__ __device__ constexpr uint32_t atc_ring()
 {
@@ -46,16 +55,17 @@ __host__ __device__ constexpr uint32_t atc_ring()
 template <int HD>
 constexpr size_t atc_smem()
 {
-	return 1024 + ((size_t)ATC_ROWS + atc_ring<HD>() * ATC_KEYS) * HD * 2;
+	return ((size_t)ATC_ROWS + atc_ring<HD>() * ATC_KEYS) * HD * 2;      // on a 1024-byte boundary
 }
 
-// K-major or N-major operand, 128-byte swizzle (8 rows of 128 bytes an atom): `lbo`
-// the distance between 64-element columns of atoms (N-major), `sbo` between 8-row
-// groups. Version 1 (sm_100).
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo)
+// Shared-memory descriptors, 128-byte swizzle (8 rows of 128 bytes an atom, 1024 bytes on to
+// the next 8 rows), version 1 (sm_100): the low word has the address and, for an
+// N-major operand, the distance between 64-element columns of atoms.
+constexpr uint32_t ATC_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+__device__ __forceinline__ uint32_t atc_desc_lo(uint32_t addr, uint32_t lbo)
 {
-	return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)((lbo >> 4) & 0x3fffu) << 16) |
-	       ((uint64_t)((sbo >> 4) & 0x3fffu) << 32) | (1ull << 46) | (2ull << 61);
+	return (addr >> 4) | ((lbo >> 4) << 16);
 }
 
 // dense kind::f16 MMA, D fp32, M = 128: A and B both fp16 (0) or both bf16 (1); B
@@ -66,23 +76,34 @@ __host__ __device__ constexpr uint32_t idesc_f16(uint32_t bf16, uint32_t n, bool
 	       ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-					   bool accumulate)
+// D (+)= A B^T, descriptors by their low words
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
+					   uint32_t accumulate)
 {
-	asm volatile("{\n\t.reg .pred p;\n\t"
-		     "setp.ne.b32 p, %4, 0;\n\t"
-		     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-		     :: "r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+	asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+		     "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+		     "setp.ne.b32 p, %5, 0;\n\t"
+		     "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
+		     :: "r"(d), "r"(a_lo), "r"(b_lo), "r"(ATC_DESC_HI), "r"(idesc), "r"(accumulate) : "memory");
 }
 
 // A from tensor memory: 16 bits a value, two a word, a row a lane
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
-					   bool accumulate)
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc,
+					   uint32_t accumulate)
 {
-	asm volatile("{\n\t.reg .pred p;\n\t"
-		     "setp.ne.b32 p, %4, 0;\n\t"
-		     "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-		     :: "r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+	asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+		     "mov.b64 b, {%2, %3};\n\t"
+		     "setp.ne.b32 p, %5, 0;\n\t"
+		     "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+		     :: "r"(d), "r"(a), "r"(b_lo), "r"(ATC_DESC_HI), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_lane()
+{
+	uint32_t r;
+	asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+	return r;
 }
 
 // 32 lanes x 32 consecutive columns
@@ -135,26 +156,28 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 {
 	constexpr uint32_t NB = atc_ring<HD>(), SLABS = HD / 64, TILE = ATC_KEYS * HD * 2;
 	constexpr uint32_t COL_S = 0, COL_O = 256;      // S (and P) 128 columns a stream, then O
-	extern __shared__ uint8_t atc_raw[];
-	__shared__ __align__(8) uint64_t b_full[NB], b_free[NB], b_q, b_s[2], b_p[2], b_o[2], b_end;
+	extern __shared__ __align__(1024) uint8_t atc_raw[];
+	__shared__ __align__(8) uint64_t b_full[NB + 1], b_free[NB + 1], b_q, b_s[2][2], b_p[2][2], b_o[2], b_end;
 	__shared__ uint32_t s_tmem, s_row[ATC_ROWS];
 	constexpr uint32_t NO_ROW = 0xffffffffu;
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-	const uint32_t q_at = (smem_addr(atc_raw) + 1023u) & ~1023u, ring = q_at + ATC_ROWS * HD * 2;
-	uint8_t *q_ptr = atc_raw + (q_at - smem_addr(atc_raw));
+	const uint32_t q_at = smem_addr(atc_raw);
+	uint8_t *q_ptr = atc_raw;
 
 	// barriers and tensor memory while the kernel before is still running
 	if (warp == 8) {
 		if (lane == 0) {
-			for (uint32_t i = 0; i < NB; i++) {
+			for (uint32_t i = 0; i <= NB; i++) {
 				mbar_init(&b_full[i], 1);
 				mbar_init(&b_free[i], 1);
 			}
 			mbar_init(&b_q, 256);
 			mbar_init(&b_end, 1);
 			for (int i = 0; i < 2; i++) {
-				mbar_init(&b_s[i], 1);
-				mbar_init(&b_p[i], 128);
+				for (int h = 0; h < 2; h++) {
+					mbar_init(&b_s[i][h], 1);
+					mbar_init(&b_p[i][h], 128);
+				}
 				mbar_init(&b_o[i], 1);
 			}
 			fence_mbar_init();
@@ -172,14 +195,17 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 	const uint32_t u = b / (kvh_n * splits);
 	b -= u * kvh_n * splits;
 	const uint32_t piece = b / kvh_n, kvh = b - piece * kvh_n;
-	uint32_t g = 0, tile = 0;
+	uint32_t tile = 0;
 	AttnGroup gr = {0, 0, 0, -1};
-	if (attn_find_unit(a, u, ATC_ROWS, &g, &tile))
-		gr = attn_group(a, g);
+	attn_find_unit(a, u, ATC_ROWS, &gr, &tile);
 	int32_t k0 = 0, k1 = gr.keys;
 	attn_piece(k0, k1, piece, splits, ATC_KEYS);
 	const uint32_t n_rows = (gr.s1 - gr.s0) * tg, row0 = tile * ATC_ROWS;
 	const bool halves = n_rows - row0 > 128;
+	const uint32_t q_slab = halves ? 256 * 128 : 128 * 128, ring = q_at + q_slab * SLABS;
+	// copy c's place in the ring, and which time round
+	auto at_of = [&](uint32_t c) { return halves ? c % NB : c % (NB + 1); };
+	auto turn_of = [&](uint32_t c) { return halves ? c / NB : c / (NB + 1); };
 	const uint32_t tiles = (uint32_t)(k1 - k0 + (int32_t)ATC_KEYS - 1) / ATC_KEYS;
 	const uint32_t pieces = a.pre_splits + a.own_splits;
 	// a row of the unit by its number among q's rows: (sequence, token, head)
@@ -190,8 +216,12 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 					     ? (s * a.n_tok + x / a.gqa) * a.n_head + kvh * a.gqa + x % a.gqa
 					     : NO_ROW;
 	}
-	// the tiles of stream i
-	auto count = [&](uint32_t i) { return halves ? tiles : (tiles + 1 - i) / 2; };
+	// the steps of stream i: its tiles' halves, but a last one without keys
+	auto count = [&](uint32_t i) {
+		const uint32_t n = halves ? tiles : (tiles + 1 - i) / 2;
+		const bool last = halves || (tiles - 1) % 2 == i;
+		return 2 * n - (last && (uint32_t)(k1 - k0) <= (tiles - 1) * ATC_KEYS + ATC_STEP);
+	};
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
@@ -221,9 +251,9 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 		for (uint32_t j = 0; j < tiles && ok; j++, page = next) {
 			next = page_of(j + 1);
 			for (int v = 0; v < 2; v++, c++) {
-				const uint32_t at = c % NB;
-				if (c >= NB)
-					ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_free[at], (c / NB - 1) & 1,
+				const uint32_t at = at_of(c), turn = turn_of(c);
+				if (turn)
+					ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_free[at], (turn - 1) & 1,
 										       WAIT_LIMIT_NS));
 				if (!ok)
 					break;
@@ -241,60 +271,85 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 		if (!ok && lane == 0)
 			*(volatile int *)a.err = ATC_ERR_RING;
 		for (uint32_t i = c > NB ? c - NB : 0; i < c; i++)
-			if (!mbar_wait_bounded(&b_full[i % NB], (i / NB) & 1, WAIT_LIMIT_NS) && lane == 0)
+			if (!mbar_wait_bounded(&b_full[at_of(i)], turn_of(i) & 1, WAIT_LIMIT_NS) && lane == 0)
 				*(volatile int *)a.err = ATC_ERR_RING;
 	} else if (warp == 8) {
-		if (lane == 0) {
+		if (elect_lane()) {
 			// ---- the MMAs
 			constexpr uint32_t BF = std::is_same<T, __nv_bfloat16>::value;
-			constexpr uint32_t id_s = idesc_f16(BF, ATC_KEYS, false), id_o = idesc_f16(BF, HD, true);
+			constexpr uint32_t id_s = idesc_f16(BF, ATC_STEP, false), id_o = idesc_f16(BF, HD, true);
 			bool ok = mbar_wait_bounded(&b_q, 0, WAIT_LIMIT_NS);
 			tc_fence_after();
-			auto scores = [&](uint32_t i, uint32_t n) {      // S of stream i's n-th tile
-				const uint32_t j = halves ? n : 2 * n + i, c = 2 * j, at = c % NB;
-				ok = ok && mbar_wait_bounded(&b_full[at], (c / NB) & 1, WAIT_LIMIT_NS);
+			const uint32_t n0 = count(0), n1 = count(1), q_next = q_slab >> 4;
+			// where each stream's next tile of K and of V is in the ring; waited for, and
+			// given back after its second half, once a tile
+			const uint32_t nb = halves ? NB : NB + 1;
+			struct Place {
+				uint32_t at, turn;
+			} kp[2] = {{0, 0}, {halves ? 0u : 2u, 0}}, vp[2] = {{1, 0}, {halves ? 1u : 3u, 0}};
+			auto advance = [&](Place &p) {
+				p.at += halves ? 2 : 4;
+				if (p.at >= nb) {
+					p.at -= nb;
+					p.turn ^= 1;
+				}
+			};
+			auto scores = [&](uint32_t i, uint32_t n) {      // S of stream i's step n
+				Place &p = kp[i];
+				if (!(n & 1))
+					ok = ok && mbar_wait_bounded(&b_full[p.at], p.turn, WAIT_LIMIT_NS);
 				if (!ok)
 					return;
-				tc_fence_after();
-				const uint32_t qa = q_at + (halves ? i * 128 * 128 : 0), ka = ring + at * TILE;
+				const uint32_t qa = atc_desc_lo(q_at + (halves ? i * 128 * 128 : 0), 16);
+				const uint32_t ka = atc_desc_lo(ring + p.at * TILE + (n & 1) * (ATC_STEP * 128), 16);
+				const uint32_t d = tmem + COL_S + i * 128 + (n & 1) * ATC_STEP;
 #pragma unroll
 				for (uint32_t k = 0; k < HD / 16; k++)
-					mma_f16_ss(tmem + COL_S + i * 128,
-						   smem_desc_sw128(qa + (k / 4) * (ATC_ROWS * 128) + (k % 4) * 32, 16, 1024),
-						   smem_desc_sw128(ka + (k / 4) * ATC_SLAB + (k % 4) * 32, 16, 1024), id_s,
-						   k != 0);
-				mma_commit(&b_s[i]);
-				if (!halves || i == 1)
-					mma_commit(&b_free[at]);
+					mma_f16_ss(d, qa + (k / 4) * q_next + (k % 4) * 2,
+						   ka + (k / 4) * (ATC_SLAB >> 4) + (k % 4) * 2, id_s, k != 0);
+				mma_commit(&b_s[i][n & 1]);
+				if (n & 1) {
+					if (!halves || i == 1)
+						mma_commit(&b_free[p.at]);
+					advance(p);
+				}
 			};
 			auto outputs = [&](uint32_t i, uint32_t n) {     // O += P V of the same
-				const uint32_t j = halves ? n : 2 * n + i, c = 2 * j + 1, at = c % NB;
-				ok = ok && mbar_wait_bounded(&b_full[at], (c / NB) & 1, WAIT_LIMIT_NS) &&
-				     mbar_wait_bounded(&b_p[i], n & 1, WAIT_LIMIT_NS);
+				Place &p = vp[i];
+				if (!(n & 1))
+					ok = ok && mbar_wait_bounded(&b_full[p.at], p.turn, WAIT_LIMIT_NS);
+				ok = ok && mbar_wait_bounded(&b_p[i][n & 1], (n / 2) & 1, WAIT_LIMIT_NS);
 				if (!ok)
 					return;
 				tc_fence_after();
-				const uint32_t va = ring + at * TILE;
+				const uint32_t va = atc_desc_lo(ring + p.at * TILE + (n & 1) * (ATC_STEP * 128), ATC_SLAB);
+				const uint32_t d = tmem + COL_O + i * HD, pa = tmem + COL_S + i * 128 + (n & 1) * ATC_STEP;
 #pragma unroll
-				for (uint32_t k = 0; k < ATC_KEYS / 16; k++)
-					mma_f16_ts(tmem + COL_O + i * HD, tmem + COL_S + i * 128 + k * 8,
-						   smem_desc_sw128(va + k * 16 * 128, ATC_SLAB, 1024), id_o, n || k);
+				for (uint32_t k = 0; k < ATC_STEP / 16; k++)
+					mma_f16_ts(d, pa + k * 8, va + k * (16 * 128 >> 4), id_o, k ? 1 : n);
 				mma_commit(&b_o[i]);
-				if (!halves || i == 1)
-					mma_commit(&b_free[at]);
+				if (n & 1) {
+					if (!halves || i == 1)
+						mma_commit(&b_free[p.at]);
+					advance(p);
+				}
 			};
-			const uint32_t n0 = count(0), n1 = count(1);
-			scores(0, 0);
-			if (n1)
-				scores(1, 0);
+			// scores two steps ahead of the outputs
+			for (uint32_t n = 0; n < 2; n++) {
+				if (n < n0)
+					scores(0, n);
+				if (n < n1)
+					scores(1, n);
+			}
+#pragma unroll 2
 			for (uint32_t n = 0; n < n0 && ok; n++) {
 				outputs(0, n);
-				if (n + 1 < n0)
-					scores(0, n + 1);
+				if (n + 2 < n0)
+					scores(0, n + 2);
 				if (n < n1)
 					outputs(1, n);
-				if (n + 1 < n1)
-					scores(1, n + 1);
+				if (n + 2 < n1)
+					scores(1, n + 2);
 			}
 			// all MMAs done before tensor memory is freed
 			mma_commit(&b_end);
@@ -319,42 +374,42 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 #pragma unroll
 			for (uint32_t e = 0; e < EACH; e++) {
 				const uint32_t r = r0 + e * (256 / QW) + threadIdx.x / QW;
-				*(uint4 *)(q_ptr + (w / 8) * (ATC_ROWS * 128) + r * 128 + (((w % 8) ^ (r & 7)) << 4)) =
+				*(uint4 *)(q_ptr + (w / 8) * q_slab + r * 128 + (((w % 8) ^ (r & 7)) << 4)) =
 					make_uint4(v[e].x ^ flip, v[e].y ^ flip, v[e].z ^ flip, v[e].w ^ flip);
 			}
 		}
-		fence_proxy_async_smem();
-		mbar_arrive(&b_q);
 
 		const uint32_t i = warp / 4, quarter = warp % 4, mine = count(i);
-		const uint32_t lanes = (quarter * 32) << 16;
+		const uint32_t lanes = (quarter * 32) << 16, my = s_row[(halves ? i * 128 : 0) + quarter * 32 + lane];
 		const uint32_t ts = tmem + lanes + COL_S + i * 128, to = tmem + lanes + COL_O + i * HD;
 		const float scale = fabsf(a.scale);
 		float m = -INFINITY, l = 0.0f;
 		bool ok = true;
+		fence_proxy_async_smem();
+		mbar_arrive(&b_q);
 		for (uint32_t n = 0; n < mine; n++) {
-			ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_s[i], n & 1, WAIT_LIMIT_NS));
+			ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_s[i][n & 1], (n / 2) & 1, WAIT_LIMIT_NS));
 			if (!ok)
 				break;
 			tc_fence_after();
-			float s[128];
-#pragma unroll
-			for (int c = 0; c < 4; c++)
-				tmem_ld32(ts + 32 * c, s + 32 * c);
+			const uint32_t tn = ts + (n & 1) * ATC_STEP;
+			float s[64];
+			tmem_ld32(tn, s);
+			tmem_ld32(tn + 32, s + 32);
 			tmem_wait_ld();
+			tmem_loaded32(s);
+			tmem_loaded32(s + 32);
+			const uint32_t j = halves ? n / 2 : 2 * (n / 2) + i;
+			const int32_t in_step = k1 - k0 - (int32_t)(j * ATC_KEYS + (n & 1) * ATC_STEP);
+			if (in_step < (int32_t)ATC_STEP) {
 #pragma unroll
-			for (int c = 0; c < 4; c++)
-				tmem_loaded32(s + 32 * c);
-			const int32_t in_tile = k1 - k0 - (int32_t)((halves ? n : 2 * n + i) * ATC_KEYS);
-			if (in_tile < (int32_t)ATC_KEYS) {
-#pragma unroll
-				for (int c = 0; c < 128; c++)
-					if (c >= in_tile)
+				for (int c = 0; c < 64; c++)
+					if (c >= in_step)
 						s[c] = -INFINITY;
 			}
 			float mx[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-			for (int c = 0; c < 128; c++)
+			for (int c = 0; c < 64; c++)
 				mx[c & 3] = fmaxf(mx[c & 3], s[c]);
 			mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 			if (n == 0) {
@@ -381,24 +436,21 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 				m = mx[0];
 			}
 			const float base = m == -INFINITY ? 0.0f : -m * scale;
-			float sum[2] = {0.0f, 0.0f};
+			float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+			uint32_t p[32];
 #pragma unroll
-			for (int h = 0; h < 2; h++) {
-				uint32_t w[32];
-#pragma unroll
-				for (int c = 0; c < 32; c++) {
-					const float x = exp2_approx(__fmaf_rn(s[64 * h + 2 * c], scale, base));
-					const float y = exp2_approx(__fmaf_rn(s[64 * h + 2 * c + 1], scale, base));
-					sum[0] += x;
-					sum[1] += y;
-					w[c] = pack_pair<T>(x, y);
-				}
-				tmem_st32(ts + 32 * h, w);
+			for (int c = 0; c < 32; c++) {
+				const float x = exp2_approx(__fmaf_rn(s[2 * c], scale, base));
+				const float y = exp2_approx(__fmaf_rn(s[2 * c + 1], scale, base));
+				sum[2 * (c & 1)] += x;
+				sum[2 * (c & 1) + 1] += y;
+				p[c] = pack_pair<T>(x, y);
 			}
-			l += sum[0] + sum[1];
+			tmem_st32(tn, p);
+			l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 			tmem_wait_st();
 			tc_fence_before();
-			mbar_arrive(&b_p[i]);
+			mbar_arrive(&b_p[i][n & 1]);
 		}
 		// all MMAs are done: the outputs go out through the ring, 32 columns of a warp's 32
 		// rows at a time, so that a row's 128 bytes leave together
@@ -407,16 +459,16 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 			*(volatile int *)a.err = ATC_ERR_ROWS;
 		if (ok) {
 			tc_fence_after();
-			const uint32_t r = (halves ? i * 128 : 0) + quarter * 32, my = s_row[r + lane];
 			const uint32_t col = 2 * piece + (halves ? 0 : i);
 			const float inv = l != 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
 			if (my != NO_ROW) {
-				float *w = a.part_w + (size_t)my * pieces + col;
-				w[0] = l != 0.0f ? (m == -INFINITY ? 0.0f : m * scale) + log2f(l) : -INFINITY;
+				float *pw = a.part_w + (size_t)my * pieces + col;
+				pw[0] = l != 0.0f ? (m == -INFINITY ? 0.0f : m * scale) + log2f(l) : -INFINITY;
 				if (halves)
-					w[1] = -INFINITY;
+					pw[1] = -INFINITY;
 			}
-			float *stage = reinterpret_cast<float *>(q_ptr + ATC_ROWS * HD * 2) + warp * (32 * 36);
+			float *stage = reinterpret_cast<float *>(q_ptr + (ring - q_at)) + warp * (32 * 36);
+#pragma unroll 1
 			for (int c = 0; mine && c < HD / 32; c++) {
 				float o[32];
 				tmem_ld32(to + 32 * c, o);
@@ -429,10 +481,11 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 				__syncwarp();
 #pragma unroll
 				for (int e = 0; e < 8; e++) {
-					const uint32_t row = e * 4 + lane / 8, at = s_row[r + row];
+					const uint32_t row = e * 4 + lane / 8, at = __shfl_sync(0xffffffffu, my, row);
 					if (at != NO_ROW)
 						*(float4 *)(a.part_o + ((size_t)at * pieces + col) * HD + 32 * c +
-							    (lane % 8) * 4) = *(float4 *)(stage + row * 36 + (lane % 8) * 4);
+							    (lane % 8) * 4) =
+							*(float4 *)(stage + row * 36 + (lane % 8) * 4);
 				}
 				__syncwarp();
 			}
