@@ -321,7 +321,6 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 		const uint32_t box = min(a.p.page, 64u), row_bytes = HD * 2;
 		uint32_t c = 0;
 		bool ok = true;
-		AttnGroup gr = {1, 0, 0, -1};           // the last group looked up: sequences [s0, s1)
 		auto push = [&](AttnStage h, const int32_t *row) {
 			const uint32_t st = c % NS, base = ring + st * R::STAGE;
 			if (c >= NS)
@@ -361,65 +360,80 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 			__syncwarp();
 			c++;
 		};
-		for (uint32_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
-			AttnStage h;
-			int32_t k0, slot;
-			uint32_t b = it, kind = 0;
-			if (b < pre_items) {
-				const uint32_t u = b / (kvh_n * a.rows_splits);
-				b -= u * kvh_n * a.rows_splits;
-				const uint32_t piece = b / kvh_n;
-				h.kvh = b - piece * kvh_n;
-				if (!attn_find_unit(a, u, ATTN_TILE_ROWS, &gr, &h.tile))
-					continue;                      // (past the last)
-				if (!gr.keys)
-					continue;
-				h.s0 = gr.s0;
-				h.n_rows = (gr.s1 - gr.s0) * tg;
-				slot = gr.slot;
-				k0 = 0;
-				h.k1 = gr.keys;
-				attn_piece(k0, h.k1, piece, a.rows_splits, ATTN_GRAIN);
-				h.slot_at = piece;
-				h.len = 0x7fffffff;
-				kind = 16;
-			} else {
-				b -= pre_items;
-				const uint32_t per = a.own_tiles * kvh_n * a.own_splits;
-				h.s0 = b / per;
-				b -= h.s0 * per;
-				h.tile = b / (kvh_n * a.own_splits);
-				b -= h.tile * kvh_n * a.own_splits;
-				const uint32_t piece = b / kvh_n;
-				h.kvh = b - piece * kvh_n;
-				h.n_rows = tg;
-				if (h.s0 < gr.s0 || h.s0 >= gr.s1)
-					gr = attn_group_of(a, h.s0);
-				h.k1 = h.len = attn_len(a, h.s0);
-				slot = __ldcg(&a.slots[h.s0]);
-				k0 = h.k1 ? gr.keys : 0;
-				kind = !piece && !k0 ? 32 : 0;          // (the first piece says so for its rows)
+		// a lane an item, 32 items' lengths and groups on their way at a time
+		for (uint64_t at = blockIdx.x; at < items && ok; at += 32ull * gridDim.x) {
+			const uint64_t it = at + (uint64_t)lane * gridDim.x;
+			const bool own = it >= pre_items && it < items;
+			const uint32_t splits = own ? a.own_splits : max(a.rows_splits, 1u);
+			uint32_t b = own ? (uint32_t)(it - pre_items) : (uint32_t)min(it, (uint64_t)items);
+			const uint32_t per = kvh_n * splits * (own ? a.own_tiles : 1);
+			AttnStage h = {};
+			h.s0 = b / per;                         // (of a prefix: the unit)
+			b -= h.s0 * per;
+			h.tile = b / (kvh_n * splits);
+			b -= h.tile * kvh_n * splits;
+			uint32_t piece = b / kvh_n;
+			h.kvh = b - piece * kvh_n;
+			h.n_rows = tg;
+			int32_t slot = own ? __ldcg(&a.slots[h.s0]) : -1, shared = 0;
+			// the groups of own items: each looked up once for all lanes in it
+			for (uint32_t left = a.n_group ? __ballot_sync(0xffffffffu, own) : 0; left;) {
+				const uint32_t s = __shfl_sync(0xffffffffu, h.s0, __ffs(left) - 1);
+				const AttnGroup gr = attn_group_of(a, s);
+				const bool in = own && (h.s0 == s || (h.s0 >= gr.s0 && h.s0 < gr.s1));
+				shared = in ? gr.keys : shared;
+				left &= ~__ballot_sync(0xffffffffu, in);
+			}
+			h.len = attn_slot_len(a, slot);
+			int32_t k0 = h.len ? shared : 0;
+			uint32_t kind = own ? (!piece && !k0 ? 32u : 0u) : 16u;  // 32: no prefix, its first piece says so
+			h.k1 = h.len;
+			h.slot_at = (own ? a.pre_splits : 0) + piece;
+			if (own)
 				attn_piece(k0, h.k1, piece, a.own_splits, a.own_grain);
-				h.slot_at = a.pre_splits + piece;
-			}
-			const uint32_t rows = min(h.n_rows - h.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS);
-			if (lane < rows && (k0 >= h.k1 || (kind & 32))) {
-				// no keys, or no prefix: the weights say so
-				const uint32_t r = h.tile * ATTN_TILE_ROWS + lane, s = h.s0 + r / tg, x = r % tg;
-				float *w = a.part_w + ((size_t)(s * a.n_tok + x / a.gqa) * a.n_head + h.kvh * a.gqa +
-						       x % a.gqa) * pieces;
-				if (k0 >= h.k1 && (!(kind & 16) || attn_len(a, s)))
-					w[h.slot_at] = -INFINITY;
-				for (uint32_t j = 0; (kind & 32) && j < a.pre_splits; j++)
-					w[j] = -INFINITY;
-			}
-			if (k0 >= h.k1)
-				continue;
-			const int32_t *row = a.p.table + (size_t)slot * a.p.max_pages;
-			for (int32_t key0 = k0; key0 < h.k1 && ok; key0 += (int32_t)R::KEYS) {
-				h.kind = (kind & 16) | (key0 == k0 ? 1u : 0u) | (key0 + (int32_t)R::KEYS >= h.k1 ? 2u : 0u);
-				h.key0 = key0;
-				push(h, row);
+			const uint64_t most = ((uint64_t)items - at + gridDim.x - 1) / gridDim.x;
+			for (uint32_t j = 0; j < (most < 32 ? (uint32_t)most : 32u) && ok; j++) {
+				AttnStage g;
+				g.s0 = __shfl_sync(0xffffffffu, h.s0, j);
+				g.tile = __shfl_sync(0xffffffffu, h.tile, j);
+				g.kvh = __shfl_sync(0xffffffffu, h.kvh, j);
+				g.n_rows = tg;
+				g.slot_at = __shfl_sync(0xffffffffu, h.slot_at, j);
+				g.k1 = __shfl_sync(0xffffffffu, h.k1, j);
+				g.len = __shfl_sync(0xffffffffu, h.len, j);
+				const uint32_t what = __shfl_sync(0xffffffffu, kind, j);
+				int32_t from = __shfl_sync(0xffffffffu, k0, j), of = __shfl_sync(0xffffffffu, slot, j);
+				if (what & 16) {
+					// a prefix's unit
+					AttnGroup gr;
+					if (!attn_find_unit(a, g.s0, ATTN_TILE_ROWS, &gr, &g.tile) || !gr.keys)
+						continue;
+					g.s0 = gr.s0;
+					g.n_rows = (gr.s1 - gr.s0) * tg;
+					g.len = 0x7fffffff;
+					of = gr.slot;
+					from = 0;
+					g.k1 = gr.keys;
+					attn_piece(from, g.k1, g.slot_at, a.rows_splits, ATTN_GRAIN);
+				}
+				const uint32_t rows = min(g.n_rows - g.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS);
+				if (lane < rows && (from >= g.k1 || (what & 32))) {
+					// no keys, or no prefix: the weights say so
+					const uint32_t r = g.tile * ATTN_TILE_ROWS + lane, s = g.s0 + r / tg, x = r % tg;
+					float *w = a.part_w + ((size_t)(s * a.n_tok + x / a.gqa) * a.n_head + g.kvh * a.gqa +
+							       x % a.gqa) * pieces;
+					if (from >= g.k1 && (!(what & 16) || attn_len(a, s)))
+						w[g.slot_at] = -INFINITY;
+					for (uint32_t i = 0; (what & 32) && i < a.pre_splits; i++)
+						w[i] = -INFINITY;
+				}
+				const int32_t *row = a.p.table + (size_t)of * a.p.max_pages;
+				for (int32_t key0 = from; key0 < g.k1 && ok; key0 += (int32_t)R::KEYS) {
+					g.kind = (what & 16) | (key0 == from ? 1u : 0u) |
+						 (key0 + (int32_t)R::KEYS >= g.k1 ? 2u : 0u);
+					g.key0 = key0;
+					push(g, row);
+				}
 			}
 		}
 		// the end; then every copy issued lands before the CTA leaves
