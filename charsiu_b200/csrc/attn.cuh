@@ -44,13 +44,13 @@ struct AttnArgs {
 	uint32_t pre_units, own_tiles;        // units of the prefix at most; row tiles a sequence
 	uint32_t rows_splits;                 // pieces of the prefix that the rows kernel makes
 	uint32_t out_type;
-	uint32_t beside;      // the prefix is another launch's, before this one: no wait for it
+	uint32_t behind;      // the rows kernel: behind the prefix's launch, no wait for it
 	float scale;          // scale * log2(e)
 	int *err;             // a wait that gave up says so here
 };
 
-// (Lengths, tables and queries are read past L1: the rows kernel may start without
-// a wait of its own, see there.)
+// (Lengths, tables and queries are read past L1: the rows kernel may start without a wait
+// of its own, see there.)
 
 // the length of a slot; 0 for none
 __device__ __forceinline__ int32_t attn_slot_len(const AttnArgs &a, int32_t slot)
@@ -243,8 +243,8 @@ __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v)
 // their way at all times. Each of a persistent grid's CTAs takes items in turn; one
 // warp runs ahead through its items (lengths, tables, then tensor copies of K and
 // V page by page, and of the item's queries) into a ring of stages, so the latency
-// of one item's start hides behind the work on the ones before. Four warps take a
-// quarter of a stage's keys each (mma.m16n8k16, scores and outputs in registers,
+// of one item's start hides behind the work on the ones before. Four warps take a quarter of a
+// stage's keys each (mma.m16n8k16, scores and outputs in registers,
 // one pass with a running maximum and sum) and are joined through the item's last
 // stage before it is given back.
 template <int HD>
@@ -254,11 +254,17 @@ struct AttnRing {
 	static constexpr uint32_t STAGES = 3;
 	static constexpr uint32_t SLAB = KEYS * 128;                // 64 elements of each key
 	static constexpr uint32_t HALF = KEYS * HD * 2;             // K, then V
+	static constexpr uint32_t STAGE = 2 * HALF;
 	static constexpr uint32_t Q_ROW = HD * 2 + 16;              // (16 bytes on: other banks)
-	static constexpr uint32_t Q_AT = 2 * HALF;
-	static constexpr uint32_t STAGE = (Q_AT + ATTN_TILE_ROWS * Q_ROW + 1023) / 1024 * 1024;
-	static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE;
+	static constexpr uint32_t Q_AT = STAGES * STAGE, Q_STAGE = ATTN_TILE_ROWS * Q_ROW;
+	static constexpr size_t SMEM = Q_AT + (size_t)STAGES * Q_STAGE;
 };
+
+// positions a tensor copy takes of one page
+__host__ __device__ inline uint32_t attn_box(uint32_t page)
+{
+	return page < 64 ? page : 64;
+}
 
 struct AttnStage {
 	uint32_t kind;        // 1: an item's first stage, 2: its last, 8: the end, 16: of a prefix
@@ -282,21 +288,21 @@ constexpr int ATTN_THREADS = (ATTN_WARPS + 1) * 32;
 constexpr int ATTN_ERR_RING = 24, ATTN_ERR_ROWS = 25;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(ATTN_THREADS)
+__global__ void __launch_bounds__(ATTN_THREADS, 2)
 attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap,
 		 const __grid_constant__ CUtensorMap vmap)
 {
 	using R = AttnRing<HD>;
 	constexpr uint32_t NS = R::STAGES;
 	constexpr int NT = HD / 8, KS = HD / 16;
-	extern __shared__ uint8_t rows_raw[];
+	extern __shared__ __align__(1024) uint8_t rows_raw[];
 	__shared__ __align__(8) uint64_t b_full[NS], b_free[NS];
 	__shared__ __align__(8) uint64_t b_join;
 	__shared__ AttnStage s_stage[NS];
 	__shared__ float s_m[ATTN_WARPS][ATTN_TILE_ROWS], s_l[ATTN_WARPS][ATTN_TILE_ROWS];
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-	const uint32_t ring = (smem_addr(rows_raw) + 1023u) & ~1023u;
-	uint8_t *ring_ptr = rows_raw + (ring - smem_addr(rows_raw));
+	const uint32_t ring = smem_addr(rows_raw);
+	uint8_t *ring_ptr = rows_raw;
 	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa, pieces = a.pre_splits + a.own_splits;
 	if (threadIdx.x == 0) {
 		for (uint32_t i = 0; i < NS; i++) {
@@ -307,10 +313,10 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 		fence_mbar_init();
 	}
 	__syncthreads();
-	// Beside the prefix's launch this one starts once all of that one's CTAs are past
-	// their own wait, so what came before both is done; what it writes, that one
-	// does not touch. It ends after that one, as the join counts on.
-	if (!a.beside)
+	// Behind the prefix's launch of the same call this one starts once all of that one's CTAs
+	// are past their own wait, so what came before both is done; what it writes, that
+	// one does not touch. It ends after that one, as the join counts on.
+	if (!a.behind)
 		pdl_wait();
 	pdl_launch_dependents();
 	const uint32_t pre_items = a.pre_units * kvh_n * a.rows_splits;
@@ -318,10 +324,12 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 
 	if (warp == ATTN_WARPS) {
 		// ---- the items, and their K, V and queries into the ring
-		const uint32_t box = min(a.p.page, 64u), row_bytes = HD * 2;
+		const uint32_t box = attn_box(a.p.page), row_bytes = HD * 2;
 		uint32_t c = 0;
 		bool ok = true;
-		auto push = [&](AttnStage h, const int32_t *row) {
+		// `ids`: pages first_page, first_page + 1, ... of the sequence, one a lane
+		constexpr uint32_t PAGES_HELD = 24;     // of 32 looked up: a stage starts in these, and has at most 8
+		auto push = [&](AttnStage h, uint32_t ids, uint32_t first_page) {
 			const uint32_t st = c % NS, base = ring + st * R::STAGE;
 			if (c >= NS)
 				ok = __all_sync(0xffffffffu,
@@ -333,11 +341,8 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 			// this lane's box: which positions, which 64 elements; K and V alike
 			const uint32_t mine = lane % (R::KEYS / 16), slab = lane / (R::KEYS / 16);
 			const uint32_t pos = (uint32_t)h.key0 + mine * box;
-			int page = (int)a.p.n_pages;            // (no page: zeros)
-			if (mine < boxes && slab < HD / 64) {
-				const uint32_t id = (uint32_t)__ldcg(&row[pos / a.p.page]);
-				page = (int)min(id, a.p.n_pages);
-			}
+			// (no page: zeros)
+			const int page = (int)min(__shfl_sync(0xffffffffu, ids, pos / a.p.page - first_page), a.p.n_pages);
 			if (lane == 0) {
 				s_stage[st] = h;
 				mbar_arrive_expect_tx(&b_full[st], 2 * boxes * box * row_bytes + q_rows * row_bytes);
@@ -354,7 +359,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 				const uint32_t r = h.tile * ATTN_TILE_ROWS + lane, s = h.s0 + r / tg, x = r % tg;
 				const T *src = (const T *)a.q + ((size_t)(s * a.n_tok + x / a.gqa) * a.n_head +
 								 h.kvh * a.gqa + x % a.gqa) * HD;
-				bulk_g2s(ring_ptr + st * R::STAGE + R::Q_AT + lane * R::Q_ROW, src, row_bytes,
+				bulk_g2s(ring_ptr + R::Q_AT + st * R::Q_STAGE + lane * R::Q_ROW, src, row_bytes,
 					 &b_full[st]);
 			}
 			__syncwarp();
@@ -391,8 +396,21 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 			h.slot_at = (own ? a.pre_splits : 0) + piece;
 			if (own)
 				attn_piece(k0, h.k1, piece, a.own_splits, a.own_grain);
-			const uint64_t most = ((uint64_t)items - at + gridDim.x - 1) / gridDim.x;
-			for (uint32_t j = 0; j < (most < 32 ? (uint32_t)most : 32u) && ok; j++) {
+			const uint32_t rows = min(tg - h.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS);
+			if (own && (k0 >= h.k1 || (kind & 32)))
+				// no keys, or no prefix: the weights say so
+				for (uint32_t i = 0; i < rows; i++) {
+					const uint32_t x = h.tile * ATTN_TILE_ROWS + i;
+					float *w = a.part_w + ((size_t)(h.s0 * a.n_tok + x / a.gqa) * a.n_head +
+							       h.kvh * a.gqa + x % a.gqa) * pieces;
+					if (k0 >= h.k1)
+						w[h.slot_at] = -INFINITY;
+					for (uint32_t j = 0; (kind & 32) && j < a.pre_splits; j++)
+						w[j] = -INFINITY;
+				}
+			uint32_t left = __ballot_sync(0xffffffffu, it < items && (!own || k0 < h.k1));
+			for (; left && ok; left &= left - 1) {
+				const int j = __ffs(left) - 1;
 				AttnStage g;
 				g.s0 = __shfl_sync(0xffffffffu, h.s0, j);
 				g.tile = __shfl_sync(0xffffffffu, h.tile, j);
@@ -415,24 +433,33 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 					from = 0;
 					g.k1 = gr.keys;
 					attn_piece(from, g.k1, g.slot_at, a.rows_splits, ATTN_GRAIN);
-				}
-				const uint32_t rows = min(g.n_rows - g.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS);
-				if (lane < rows && (from >= g.k1 || (what & 32))) {
-					// no keys, or no prefix: the weights say so
 					const uint32_t r = g.tile * ATTN_TILE_ROWS + lane, s = g.s0 + r / tg, x = r % tg;
-					float *w = a.part_w + ((size_t)(s * a.n_tok + x / a.gqa) * a.n_head + g.kvh * a.gqa +
-							       x % a.gqa) * pieces;
-					if (from >= g.k1 && (!(what & 16) || attn_len(a, s)))
-						w[g.slot_at] = -INFINITY;
-					for (uint32_t i = 0; (what & 32) && i < a.pre_splits; i++)
-						w[i] = -INFINITY;
+					if (from >= g.k1 && lane < ATTN_TILE_ROWS && r < g.n_rows && attn_len(a, s))
+						a.part_w[((size_t)(s * a.n_tok + x / a.gqa) * a.n_head + g.kvh * a.gqa +
+							  x % a.gqa) * pieces + g.slot_at] = -INFINITY;
 				}
 				const int32_t *row = a.p.table + (size_t)of * a.p.max_pages;
+				uint32_t ids = 0, more = 0, at_page = 0;
+				const uint32_t pages = g.k1 > from ? (uint32_t)(g.k1 - 1) / a.p.page + 1 : 0;
+				auto pages_from = [&](uint32_t p) {
+					return p + lane < pages ? (uint32_t)__ldcg(&row[p + lane]) : 0u;
+				};
+				if (from < g.k1) {
+					at_page = (uint32_t)from / a.p.page;
+					ids = pages_from(at_page);
+					more = pages_from(at_page + PAGES_HELD);
+				}
 				for (int32_t key0 = from; key0 < g.k1 && ok; key0 += (int32_t)R::KEYS) {
 					g.kind = (what & 16) | (key0 == from ? 1u : 0u) |
 						 (key0 + (int32_t)R::KEYS >= g.k1 ? 2u : 0u);
 					g.key0 = key0;
-					push(g, row);
+					// (a stage's pages lie within 32 from at_page on)
+					while ((uint32_t)key0 / a.p.page >= at_page + PAGES_HELD) {
+						at_page += PAGES_HELD;
+						ids = more;
+						more = pages_from(at_page + PAGES_HELD);
+					}
+					push(g, ids, at_page);
 				}
 			}
 		}
@@ -440,7 +467,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 		AttnStage end = {};
 		end.kind = 8;
 		if (ok)
-			push(end, nullptr);
+			push(end, 0, 0);
 		if (!ok && lane == 0)
 			*(volatile int *)a.err = ATTN_ERR_RING;
 		for (uint32_t i = c > NS ? c - NS : 0; i < c; i++)
@@ -485,7 +512,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 				least = min(min(__reduce_min_sync(0xffffffffu, limit[0]),
 						__reduce_min_sync(0xffffffffu, limit[1])), h.k1);
 				const uint32_t rows = min(h.n_rows - h.tile * ATTN_TILE_ROWS, ATTN_TILE_ROWS);
-				const uint8_t *qs = ring_ptr + st * R::STAGE + R::Q_AT;
+				const uint8_t *qs = ring_ptr + R::Q_AT + st * R::Q_STAGE;
 #pragma unroll
 				for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -700,7 +727,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 		if (!ended && lane == 0)
 			*(volatile int *)a.err = ATTN_ERR_ROWS;
 	}
-	if (a.beside)
+	if (a.behind)
 		pdl_wait();
 }
 

@@ -43,9 +43,7 @@ constexpr uint32_t ATC_STEP = 64;                    // keys of a step: half a t
 constexpr int ATC_THREADS = 320;
 constexpr uint32_t ATC_SLAB = ATC_KEYS * 128;        // 128 rows of 64 elements
 
-// Tiles in the ring: what fits beside Q; one more where Q is 128 rows (a half of it is a
-// tile). Streams on the same rows need it: scores run two steps ahead of outputs, so
-// the second stream asks for K of tile 3 while V of tile 0 is still to be used.
+// Tiles in the ring: what fits beside Q; one more where Q is 128 rows (a half of it is a tile)
 template <int HD>
 __host__ __device__ constexpr uint32_t atc_ring()
 {
@@ -234,12 +232,13 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 			w[0] = w[1] = -INFINITY;
 		}
 	} else if (warp == 9) {
-		// ---- K and V tiles into the ring: K of tile j is copy 2 j, V copy 2 j + 1
-		const uint32_t box = min(a.p.page, 64u), per = ATC_KEYS / box;     // positions; boxes a tile
+		// ---- K and V tiles into the ring, in the order in which they are asked for: a tile's K,
+		// then its V; of two streams on the same rows, both their K first
+		const uint32_t box = attn_box(a.p.page), per = ATC_KEYS / box;     // positions; boxes a tile
 		const int32_t *row = a.p.table + (size_t)gr.slot * a.p.max_pages;
 		const uint32_t my_box = lane % per, my_slab = lane / per;
 		bool ok = true;
-		uint32_t c = 0;
+		uint32_t c = 0, issued = 0, turns = 0;           // (bits by place: copied to, the turn's parity)
 		// a page past the piece, or no page at all, reads as zeros
 		auto pos_of = [&](uint32_t j) { return (uint32_t)k0 + j * ATC_KEYS + my_box * box; };
 		auto page_of = [&](uint32_t j) {
@@ -247,10 +246,14 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 			const uint32_t page = pos < (uint32_t)k1 ? (uint32_t)__ldcg(&row[pos / a.p.page]) : a.p.n_pages;
 			return (int)min(page, a.p.n_pages);
 		};
-		int page = page_of(0), next = 0;
-		for (uint32_t j = 0; j < tiles && ok; j++, page = next) {
-			next = page_of(j + 1);
-			for (int v = 0; v < 2; v++, c++) {
+		const uint32_t group = halves ? 1 : 2;
+		int page[2] = {page_of(0), page_of(1)};
+		for (uint32_t j = 0; j < tiles && ok; j += group) {
+			const int next[2] = {page_of(j + group), page_of(j + group + 1)};
+			for (uint32_t x = 0; x < 2 * group; x++, c++) {
+				const uint32_t v = x / group, t = x % group;
+				if (j + t >= tiles)
+					continue;                  // (of the last pair, where tiles is odd)
 				const uint32_t at = at_of(c), turn = turn_of(c);
 				if (turn)
 					ok = __all_sync(0xffffffffu, mbar_wait_bounded(&b_free[at], (turn - 1) & 1,
@@ -263,15 +266,20 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 				if (my_slab < SLABS)
 					tma_load_4d(ring + at * TILE + my_slab * ATC_SLAB + my_box * box * 128,
 						    v ? &vmap : &kmap, (int)(my_slab * 64),
-						    (int)(pos_of(j) % a.p.page), (int)kvh, page, &b_full[at]);
+						    (int)(pos_of(j + t) % a.p.page), (int)kvh, page[t], &b_full[at]);
 				__syncwarp();
+				issued |= 1u << at;
+				turns = (turns & ~(1u << at)) | (turn & 1) << at;
 			}
+			page[0] = next[0];
+			page[1] = next[1];
 		}
 		// every copy issued lands before the CTA leaves (already so unless a wait gave up)
 		if (!ok && lane == 0)
 			*(volatile int *)a.err = ATC_ERR_RING;
-		for (uint32_t i = c > NB ? c - NB : 0; i < c; i++)
-			if (!mbar_wait_bounded(&b_full[at_of(i)], turn_of(i) & 1, WAIT_LIMIT_NS) && lane == 0)
+		for (uint32_t i = 0; i <= NB; i++)
+			if ((issued >> i & 1) && !mbar_wait_bounded(&b_full[i], turns >> i & 1, WAIT_LIMIT_NS) &&
+			    lane == 0)
 				*(volatile int *)a.err = ATC_ERR_RING;
 	} else if (warp == 8) {
 		if (elect_lane()) {
@@ -286,7 +294,7 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 			const uint32_t nb = halves ? NB : NB + 1;
 			struct Place {
 				uint32_t at, turn;
-			} kp[2] = {{0, 0}, {halves ? 0u : 2u, 0}}, vp[2] = {{1, 0}, {halves ? 1u : 3u, 0}};
+			} kp[2] = {{0, 0}, {halves ? 0u : 1u, 0}}, vp[2] = {{halves ? 1u : 2u, 0}, {halves ? 1u : 3u, 0}};
 			auto advance = [&](Place &p) {
 				p.at += halves ? 2 : 4;
 				if (p.at >= nb) {

@@ -80,7 +80,8 @@ bool launch(charsiu_gpu *g, void *stream, K kernel, dim3 grid, unsigned block, s
 	return true;
 }
 
-// more than 48 KB of shared memory, asked for once a kernel and device
+// more than 48 KB of shared memory, asked for once a kernel and device; and the whole of a
+// multiprocessor's as shared memory, so that CTAs of different kernels find room on one
 template <typename K>
 bool allow_smem(charsiu_gpu *g, K kernel, size_t bytes, uint64_t &done)
 {
@@ -88,7 +89,9 @@ bool allow_smem(charsiu_gpu *g, K kernel, size_t bytes, uint64_t &done)
 	if (done & bit)
 		return true;
 	if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
-	    cudaSuccess) {
+		    cudaSuccess ||
+	    cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+				 cudaSharedmemCarveoutMaxShared) != cudaSuccess) {
 		cudaGetLastError();
 		layer_whine(g, "a kernel's shared memory was refused");
 		return false;
@@ -234,8 +237,8 @@ size_t attention_bytes(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu
 	return (size_t)(parts * b->n_tok * b->n_head * (p->head_dim + 1) * sizeof(float) + 15) / 16 * 16;
 }
 
-// K or V of one layer as (element, position, head, page); boxes of 64 elements and at
-// most 64 positions of a page. A dimension of one element has no stride to speak of.
+// K or V of one layer as (element, position, head, page); boxes of 64 elements and
+// attn_box positions of a page. A dimension of one element has no stride to speak of.
 bool attention_map(CUtensorMap *map, const charsiu_gpu_pages *p, const void *base, unsigned layer)
 {
 	const auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encode());
@@ -245,7 +248,7 @@ bool attention_map(CUtensorMap *map, const charsiu_gpu_pages *p, const void *bas
 	const cuuint64_t row = 2ull * p->head_dim;
 	const cuuint64_t strides[3] = {2 * p->pos_stride, p->n_head_kv > 1 ? 2 * p->head_stride : row,
 				       p->n_pages > 1 ? 2 * p->page_stride : row};
-	const cuuint32_t box[4] = {64, p->page < 64 ? p->page : 64, 1, 1}, ones[4] = {1, 1, 1, 1};
+	const cuuint32_t box[4] = {64, attn_box(p->page), 1, 1}, ones[4] = {1, 1, 1, 1};
 	return enc(map, p->type == TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
 		   4, (uint8_t *)const_cast<void *>(base) + 2 * layer * p->layer_stride, dims, strides, box, ones,
 		   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -262,13 +265,13 @@ int attention(charsiu_gpu *g, AttnArgs &a, bool tc, void *stream)
 	if (!allow_smem(g, attn_rows_kernel<T, HD>, AttnRing<HD>::SMEM, smem_done) ||
 	    !allow_smem(g, attn_tc_kernel<T, HD>, atc_smem<HD>(), tc_done))
 		return -1;
+	if (tc && !launch(g, stream, attn_tc_kernel<T, HD>,
+			  dim3(a.pre_units * a.p.n_head_kv * (a.pre_splits / 2)), ATC_THREADS, atc_smem<HD>(), a,
+			  kmap, vmap))
+		return -1;
 	if (tc) {
-		if (!launch(g, stream, attn_tc_kernel<T, HD>,
-			    dim3(a.pre_units * a.p.n_head_kv * (a.pre_splits / 2)), ATC_THREADS, atc_smem<HD>(), a,
-			    kmap, vmap))
-			return -1;
-		a.beside = 1;
 		a.pre_units = 0;
+		a.behind = 1;
 	}
 	const uint64_t items = (uint64_t)a.p.n_head_kv * ((uint64_t)a.pre_units * a.rows_splits +
 							  (uint64_t)a.n_seq * a.own_tiles * a.own_splits);
