@@ -531,6 +531,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 #pragma unroll
 				for (int j = 0; j < NK; j++) {
 					s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+					float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // (two chains of MMAs, not one)
 					const uint32_t key = w0 + j * 8 + (lane & 7);
 #pragma unroll
 					for (int k2 = 0; k2 < KS / 2; k2++) {
@@ -538,8 +539,11 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 						uint32_t kb[4];
 						ldmatrix_x4(kb, ks_ + (w / 8) * R::SLAB + key * 128 + (((w % 8) ^ (key & 7)) << 4));
 						mma_16816<T>(s[j], qa[2 * k2], kb[0], kb[1]);
-						mma_16816<T>(s[j], qa[2 * k2 + 1], kb[2], kb[3]);
+						mma_16816<T>(odd, qa[2 * k2 + 1], kb[2], kb[3]);
 					}
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						s[j][e] += odd[e];
 				}
 				const bool ragged = key0 + (int32_t)R::WKEYS > least;
 				float mx[2] = {m[0], m[1]};

@@ -444,18 +444,18 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 				m = mx[0];
 			}
 			const float base = m == -INFINITY ? 0.0f : -m * scale;
-			float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+			const uint64_t scale2 = pack2(scale, scale), base2 = pack2(base, base);
+			uint64_t sum[2] = {0, 0};                // pairs of sums
 			uint32_t p[32];
 #pragma unroll
 			for (int c = 0; c < 32; c++) {
-				const float x = exp2_approx(__fmaf_rn(s[2 * c], scale, base));
-				const float y = exp2_approx(__fmaf_rn(s[2 * c + 1], scale, base));
-				sum[2 * (c & 1)] += x;
-				sum[2 * (c & 1) + 1] += y;
-				p[c] = pack_pair<T>(x, y);
+				const uint64_t x = fma2_rn(pack2(s[2 * c], s[2 * c + 1]), scale2, base2);
+				const float e0 = exp2_approx(lo2(x)), e1 = exp2_approx(hi2(x));
+				sum[c & 1] = add2_rn(sum[c & 1], pack2(e0, e1));
+				p[c] = pack_pair<T>(e0, e1);
 			}
 			tmem_st32(tn, p);
-			l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+			l += (lo2(sum[0]) + hi2(sum[0])) + (lo2(sum[1]) + hi2(sum[1]));
 			tmem_wait_st();
 			tc_fence_before();
 			mbar_arrive(&b_p[i][n & 1]);
