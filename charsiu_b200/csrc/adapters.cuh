@@ -3,11 +3,12 @@
 // (charsiu_gpu_adapters_dev): y_r = base_r + scale_a B_a (A_a x_r), a = which[r].
 //
 // Two launches. The first makes t_r = A_a x_r (rank numbers a row): K is cut into
-// pieces, one a CTA, whose sums go to scratch. The second adds the pieces up and
-// makes y. Both take tiles of 16 rows, as mma.sync's m; a tile's rows may want
-// different adapters, so a tile goes over the distinct ones among its rows, each
-// product made into accumulators of its own and kept only for the rows that want
-// it (whatever an adapter's weights are, they reach no other row).
+// pieces whose sums go to scratch. The second adds the pieces up and makes y. Both
+// take tiles of 16 rows, as mma.sync's m. A tile's rows may want different adapters:
+// each of its distinct ones is a product of its own over all 16 rows, of which only
+// the rows that want it are kept (so whatever an adapter's weights are, they reach no
+// other row). In a long prompt a tile has one; in a decode step of many requests they
+// are spread over warps and CTAs.
 //
 // Bound by memory: an adapter's weights are used for few rows, and y is read and
 // written for rank / 4 multiply-adds a byte.
@@ -45,21 +46,20 @@ struct AdaptArgs {
 	const float *d;
 	const int32_t *which;
 	float *t;               // [set][piece][row][RT]
-	uint32_t n_sets, m, k, pieces, blocks;
+	uint32_t n_sets, m, k;
+	uint32_t pieces;        // of K
+	uint32_t parts;         // the first launch: CTAs that share a tile's distinct adapters
+	uint32_t cols;          // the second: columns a CTA, a multiple of 32
+	uint32_t blocks;        // and CTAs over all sets' columns
 };
 
-// The next distinct adapter of the tile after those in `done` (bits of rows): its
-// number, and the rows that want it; -1 none. `mine` is the adapter of row lane % 16.
-__device__ __forceinline__ int32_t adapt_next(int32_t mine, uint32_t &done, uint32_t *rows)
-{
-	const uint32_t left = __ballot_sync(0xffffffffu, mine >= 0) & ~done & 0xffffu;
-	if (!left)
-		return -1;
-	const int32_t a = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
-	*rows = __ballot_sync(0xffffffffu, mine == a) & 0xffffu;
-	done |= *rows;
-	return a;
-}
+// A tile's distinct adapters: number, rows (a bit each), rank and scale
+struct AdaptTile {
+	int32_t ad[ADAPT_ROWS];
+	uint32_t rows[ADAPT_ROWS], rank[ADAPT_ROWS];
+	float scale[ADAPT_ROWS];
+	uint32_t n, wants;      // how many; the rows that want one
+};
 
 __device__ __forceinline__ int32_t adapt_which(const AdaptArgs &a, const AdaptSet &s, uint32_t row)
 {
@@ -73,6 +73,28 @@ __device__ __forceinline__ uint32_t adapt_rank(const AdaptSet &s, int32_t a)
 {
 	const int32_t r = s.rank[a];
 	return r < 0 ? 0 : (uint32_t)r > s.max_rank ? s.max_rank : (uint32_t)r;
+}
+
+// by one warp
+__device__ __forceinline__ void adapt_tile(const AdaptArgs &a, const AdaptSet &s, uint32_t row0,
+					   AdaptTile &t)
+{
+	const uint32_t lane = threadIdx.x & 31;
+	const int32_t mine = lane < ADAPT_ROWS ? adapt_which(a, s, row0 + lane) : -1;
+	const uint32_t same = __match_any_sync(0xffffffffu, mine);
+	const bool first = mine >= 0 && (int)lane == __ffs(same) - 1;
+	const uint32_t firsts = __ballot_sync(0xffffffffu, first), wants = __ballot_sync(0xffffffffu, mine >= 0);
+	if (first) {
+		const uint32_t at = __popc(firsts & ((1u << lane) - 1));
+		t.ad[at] = mine;
+		t.rows[at] = same;
+		t.rank[at] = adapt_rank(s, mine);
+		t.scale[at] = s.scale[mine];
+	}
+	if (lane == 0) {
+		t.n = __popc(firsts);
+		t.wants = wants;
+	}
 }
 
 // two int8 of a word as a pair of T
@@ -93,84 +115,130 @@ adapt_shrink_kernel(const __grid_constant__ AdaptArgs a)
 {
 	constexpr int NT = RT / 8;
 	__shared__ float s_t[ADAPT_WARPS][ADAPT_ROWS][RT];
+	__shared__ AdaptTile s_tile;
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
-	const uint32_t row0 = blockIdx.x * ADAPT_ROWS, piece = blockIdx.y;
+	const uint32_t row0 = blockIdx.x * ADAPT_ROWS, piece = blockIdx.y / a.parts, part = blockIdx.y % a.parts;
 	const AdaptSet &set = a.s[blockIdx.z];
 	pdl_wait();
 	pdl_launch_dependents();
+	if (warp == 0)
+		adapt_tile(a, set, row0, s_tile);
+	__syncthreads();
 	const uint32_t nb = a.k / 32, each = (nb + a.pieces - 1) / a.pieces;
-	const uint32_t b0 = piece * each, b1 = min(b0 + each, nb);
-	const int32_t mine = adapt_which(a, set, row0 + (lane & 15));
-	float keep[NT][4];
+	const uint32_t b0 = min(piece * each, nb), b1 = min(b0 + each, nb);
+	const int8_t *xq[2];
+	const float *xd[2];
+	bool real[2];
 #pragma unroll
-	for (int n = 0; n < NT; n++)
-		keep[n][0] = keep[n][1] = keep[n][2] = keep[n][3] = 0.0f;
-	uint32_t done = 0, rows;
-	for (int32_t ad; (ad = adapt_next(mine, done, &rows)) >= 0;) {
-		const uint32_t rank = adapt_rank(set, ad);
-		const T *w = (const T *)set.a + (size_t)ad * set.max_rank * a.k;
+	for (int h = 0; h < 2; h++) {
+		const uint32_t r = row0 + lane / 4 + 8 * h;
+		real[h] = r < a.m;
+		xq[h] = a.q + (size_t)(real[h] ? r : row0) * a.k + c * 8;
+		xd[h] = a.d + (size_t)(real[h] ? r : row0) * nb;
+	}
+	for (uint32_t j = part; j < s_tile.n; j += a.parts) {
+		const uint32_t rank = s_tile.rank[j], rows = s_tile.rows[j];
+		const T *w = (const T *)set.a + ((size_t)s_tile.ad[j] * set.max_rank + lane / 4) * a.k + c * 8;
 		float acc[NT][4];
 #pragma unroll
 		for (int n = 0; n < NT; n++)
 			acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-		for (uint32_t b = b0 + warp; b < b1; b += ADAPT_WARPS) {
-			uint32_t x[2][2] = {{0, 0}, {0, 0}};
-			float dd[2] = {0.0f, 0.0f};
+		// the next block's loads go out before this one's products
+		struct Block {
+			uint2 x[2];
+			float d[2];
+			uint4 w[NT];
+		};
+		auto load = [&](Block &k, uint32_t b) {
 #pragma unroll
 			for (int h = 0; h < 2; h++) {
-				const uint32_t r = row0 + lane / 4 + 8 * h;
-				if (r < a.m) {
-					const uint2 v = *(const uint2 *)(a.q + (size_t)r * a.k + b * 32 + c * 8);
-					x[h][0] = v.x;
-					x[h][1] = v.y;
-					dd[h] = a.d[(size_t)r * nb + b];
-				}
+				k.x[h] = real[h] ? *(const uint2 *)(xq[h] + b * 32) : make_uint2(0, 0);
+				k.d[h] = real[h] ? xd[h][b] : 0.0f;
 			}
+#pragma unroll
+			for (int n = 0; n < NT; n++)
+				k.w[n] = n * 8 + lane / 4 < rank ? *(const uint4 *)(w + (size_t)n * 8 * a.k + b * 32)
+								 : make_uint4(0, 0, 0, 0);
+		};
+		Block now, next;
+		if (b0 + warp < b1)
+			load(now, b0 + warp);
+		for (uint32_t b = b0 + warp; b < b1; b += ADAPT_WARPS) {
+			if (b + ADAPT_WARPS < b1)
+				load(next, b + ADAPT_WARPS);
 			uint32_t fa[2][4];
 #pragma unroll
 			for (int s = 0; s < 2; s++) {
-				fa[s][0] = int8_pair<T>(x[0][s], 0);
-				fa[s][1] = int8_pair<T>(x[1][s], 0);
-				fa[s][2] = int8_pair<T>(x[0][s], 2);
-				fa[s][3] = int8_pair<T>(x[1][s], 2);
+				const uint32_t x0 = s ? now.x[0].y : now.x[0].x, x1 = s ? now.x[1].y : now.x[1].x;
+				fa[s][0] = int8_pair<T>(x0, 0);
+				fa[s][1] = int8_pair<T>(x1, 0);
+				fa[s][2] = int8_pair<T>(x0, 2);
+				fa[s][3] = int8_pair<T>(x1, 2);
 			}
 #pragma unroll
 			for (int n = 0; n < NT; n++) {
-				const uint32_t r = n * 8 + lane / 4;
-				uint4 v = make_uint4(0, 0, 0, 0);
-				if (r < rank)
-					v = *(const uint4 *)(w + (size_t)r * a.k + b * 32 + c * 8);
-				float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-				mma_16816<T>(part, fa[0], v.x, v.y);
-				mma_16816<T>(part, fa[1], v.z, v.w);
+				float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+				mma_16816<T>(sum, fa[0], now.w[n].x, now.w[n].y);
+				mma_16816<T>(sum, fa[1], now.w[n].z, now.w[n].w);
 #pragma unroll
 				for (int e = 0; e < 4; e++)
-					acc[n][e] = __fmaf_rn(dd[e >> 1], part[e], acc[n][e]);
+					acc[n][e] = __fmaf_rn(now.d[e >> 1], sum[e], acc[n][e]);
 			}
+			now = next;
 		}
+		__syncthreads();                  // (the last adapter's sums have been read)
 #pragma unroll
 		for (int n = 0; n < NT; n++)
 #pragma unroll
-			for (int e = 0; e < 4; e++)
-				if (rows >> (lane / 4 + 8 * (e >> 1)) & 1)
-					keep[n][e] = acc[n][e];
+			for (int e = 0; e < 4; e += 2)
+				*(float2 *)&s_t[warp][lane / 4 + 4 * e][n * 8 + c * 2] = make_float2(acc[n][e], acc[n][e + 1]);
+		__syncthreads();
+		float *t = a.t + (((size_t)blockIdx.z * a.pieces + piece) * a.m + row0) * RT;
+		for (uint32_t i = threadIdx.x; i < ADAPT_ROWS * RT; i += ADAPT_WARPS * 32) {
+			float v = 0.0f;
+#pragma unroll
+			for (int x = 0; x < (int)ADAPT_WARPS; x++)
+				v += s_t[x][i / RT][i % RT];
+			if (rows >> (i / RT) & 1)
+				t[i] = v;
+		}
 	}
+}
+
+// Rows row0 + r of y, r a bit of `rows`, columns [col0, end): the base's bits, by threads
+// `at` of `n`; eight on their way at a time. (One after another, a prompt without an
+// adapter between others took the whole launch 60 us.)
+__device__ __forceinline__ void adapt_copy(const AdaptSet &s, uint32_t row0, uint32_t rows, uint32_t col0,
+					   uint32_t end, uint32_t at, uint32_t n)
+{
+	if (!rows || s.base == s.y)
+		return;
+	const bool fours = s.n % 4 == 0 && !(((uintptr_t)s.base | (uintptr_t)s.y) & 15);
+	const uint32_t each = fours ? 4 : 1, wide = (end - col0) / each, words = ADAPT_ROWS * wide;
+	for (uint32_t x0 = at; x0 < words; x0 += 8 * n) {
+		float4 v[8];
 #pragma unroll
-	for (int n = 0; n < NT; n++)
+		for (int j = 0; j < 8; j++) {
+			const uint32_t x = x0 + j * n, r = x / wide, c = col0 + (x - r * wide) * each;
+			if (x < words && (rows >> r & 1)) {
+				const float *b = s.base + (size_t)(row0 + r) * s.n + c;
+				if (fours)
+					v[j] = *(const float4 *)b;
+				else
+					v[j].x = *b;
+			}
+		}
 #pragma unroll
-		for (int e = 0; e < 4; e++)
-			s_t[warp][lane / 4 + 8 * (e >> 1)][n * 8 + c * 2 + (e & 1)] = keep[n][e];
-	__syncthreads();
-	float *t = a.t + (((size_t)blockIdx.z * a.pieces + piece) * a.m + row0) * RT;
-	for (uint32_t i = threadIdx.x; i < ADAPT_ROWS * RT; i += ADAPT_WARPS * 32) {
-		const uint32_t r = i / RT;
-		if (row0 + r >= a.m)
-			break;
-		float v = 0.0f;
-#pragma unroll
-		for (int w = 0; w < (int)ADAPT_WARPS; w++)
-			v += s_t[w][r][i % RT];
-		t[i] = v;
+		for (int j = 0; j < 8; j++) {
+			const uint32_t x = x0 + j * n, r = x / wide, c = col0 + (x - r * wide) * each;
+			if (x < words && (rows >> r & 1)) {
+				float *y = s.y + (size_t)(row0 + r) * s.n + c;
+				if (fours)
+					*(float4 *)y = v[j];
+				else
+					*y = v[j].x;
+			}
+		}
 	}
 }
 
@@ -183,35 +251,46 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
 		     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// y of one tile of rows and ADAPT_COLS columns of one set: each warp 8-column groups.
-// The ranks are permuted alike for t and B so that a lane's RT / 4 are consecutive.
-constexpr uint32_t ADAPT_COLS = 128;
-
+// y of one tile of rows and a.cols columns of one set. An item of work is a distinct
+// adapter of the tile and 8 columns; the warps take them in turn, the next one's loads
+// on their way before this one's products. The ranks are permuted alike for t and B so
+// that a lane's RT / 4 are consecutive.
 template <typename T, int RT>
 __global__ void __launch_bounds__(ADAPT_WARPS * 32)
 adapt_expand_kernel(const __grid_constant__ AdaptArgs a)
 {
 	constexpr int SP = RT / 4, KS = RT / 8;          // ranks a lane; k steps
 	__shared__ float s_t[ADAPT_ROWS][RT];
+	__shared__ AdaptTile s_tile;
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
 	const uint32_t row0 = blockIdx.x * ADAPT_ROWS;
 	uint32_t si = 0;
 	while (blockIdx.y >= a.s[si].block_end)
 		si++;
 	const AdaptSet &set = a.s[si];
-	const uint32_t col0 = (blockIdx.y - (si ? a.s[si - 1].block_end : 0)) * ADAPT_COLS;
+	const uint32_t col0 = (blockIdx.y - (si ? a.s[si - 1].block_end : 0)) * a.cols;
 	pdl_wait();
 	pdl_launch_dependents();
-	const int32_t mine = adapt_which(a, set, row0 + (lane & 15));
-	const uint32_t wants = __ballot_sync(0xffffffffu, mine >= 0);
-	for (uint32_t i = threadIdx.x; i < ADAPT_ROWS * RT; i += ADAPT_WARPS * 32) {
-		float v = 0.0f;
-		if (row0 + i / RT < a.m)
+	if (warp == 0)
+		adapt_tile(a, set, row0, s_tile);
+	{
+		const float *t = a.t + ((size_t)si * a.pieces * a.m + row0) * RT;
+		const uint32_t filled = min(a.m - row0, ADAPT_ROWS) * RT;
+		for (uint32_t i = threadIdx.x; i < ADAPT_ROWS * RT; i += ADAPT_WARPS * 32) {
+			float v = 0.0f;
+#pragma unroll 4
 			for (uint32_t p = 0; p < a.pieces; p++)
-				v += a.t[(((size_t)si * a.pieces + p) * a.m + row0) * RT + i];
-		s_t[i / RT][i % RT] = v;
+				v += i < filled ? t[(size_t)p * a.m * RT + i] : 0.0f;
+			s_t[i / RT][i % RT] = v;          // (rows that want no adapter: never used)
+		}
 	}
 	__syncthreads();
+	const uint32_t end = min(col0 + a.cols, set.n), groups = (end - col0 + 7) / 8;
+	// two columns a load and store
+	const bool pairs = set.n % 2 == 0 && !(((uintptr_t)set.base | (uintptr_t)set.y) & 7);
+	// rows of no adapter keep the base's bits
+	const uint32_t there = a.m - row0 < ADAPT_ROWS ? (1u << (a.m - row0)) - 1 : 0xffffu;
+	adapt_copy(set, row0, there & ~s_tile.wants, col0, end, threadIdx.x, ADAPT_WARPS * 32);
 	uint32_t hi[KS][4], lo[KS][4];
 #pragma unroll
 	for (int ks = 0; ks < KS; ks++)
@@ -221,49 +300,427 @@ adapt_expand_kernel(const __grid_constant__ AdaptArgs a)
 			hi[ks][j] = __float_as_uint(v) & 0xffffe000u;
 			lo[ks][j] = __float_as_uint(__fsub_rn(v, __uint_as_float(hi[ks][j])));
 		}
-	for (uint32_t n0 = col0 + warp * 8; n0 < min(col0 + ADAPT_COLS, set.n); n0 += ADAPT_WARPS * 8) {
-		float keep[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-		uint32_t done = 0, rows;
-		for (int32_t ad; (ad = adapt_next(mine, done, &rows)) >= 0;) {
-			const uint32_t rank = adapt_rank(set, ad);
-			const float scale = set.scale[ad];
-			const uint32_t n = n0 + lane / 4;
-			T w[SP];
+	struct Item {
+		uint32_t w[SP / 2];
+		float base[4];
+	};
+	auto load = [&](Item &it, uint32_t item) {
+		const uint32_t j = item / groups, n0 = col0 + (item - j * groups) * 8, n = n0 + lane / 4;
+		const uint32_t rank = s_tile.rank[j], rows = s_tile.rows[j];
+		const T *src = (const T *)set.b + ((size_t)s_tile.ad[j] * set.n + n) * set.max_rank + c * SP;
 #pragma unroll
-			for (int j = 0; j < SP; j += SP < 8 ? SP : 8) {
-				const T *src = (const T *)set.b + ((size_t)ad * set.n + n) * set.max_rank + c * SP + j;
-				const bool ok = n < set.n && c * SP + j < rank;
-				if (SP == 2) {
-					*(uint32_t *)(w + j) = ok ? *(const uint32_t *)src : 0u;
-				} else if (SP == 4) {
-					*(uint2 *)(w + j) = ok ? *(const uint2 *)src : make_uint2(0, 0);
-				} else {
-					*(uint4 *)(w + j) = ok ? *(const uint4 *)src : make_uint4(0, 0, 0, 0);
+		for (int x = 0; x < SP; x += SP < 8 ? SP : 8) {
+			const bool ok = n < set.n && c * SP + x < rank;
+			if (SP == 2) {
+				it.w[0] = ok ? *(const uint32_t *)src : 0u;
+			} else if (SP == 4) {
+				*(uint2 *)it.w = ok ? *(const uint2 *)src : make_uint2(0, 0);
+			} else {
+				*(uint4 *)(it.w + x / 2) = ok ? *(const uint4 *)(src + x) : make_uint4(0, 0, 0, 0);
+			}
+		}
+#pragma unroll
+		for (int h = 0; h < 2; h++) {
+			const uint32_t r = lane / 4 + 8 * h, col = n0 + c * 2;
+			const float *b = set.base + (size_t)(row0 + r) * set.n + col;
+			it.base[2 * h] = it.base[2 * h + 1] = 0.0f;
+			if (rows >> r & 1) {
+				if (pairs && col < set.n) {
+					const float2 v = *(const float2 *)b;
+					it.base[2 * h] = v.x;
+					it.base[2 * h + 1] = v.y;
+				} else if (col < set.n) {
+					it.base[2 * h] = b[0];
+					it.base[2 * h + 1] = col + 1 < set.n ? b[1] : 0.0f;
 				}
 			}
-			float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+		}
+	};
+	const uint32_t items = s_tile.n * groups;
+	Item now, next;
+	if (warp < items)
+		load(now, warp);
+	for (uint32_t item = warp; item < items; item += ADAPT_WARPS) {
+		if (item + ADAPT_WARPS < items)
+			load(next, item + ADAPT_WARPS);
+		const uint32_t j = item / groups, n0 = col0 + (item - j * groups) * 8;
+		const uint32_t rank = s_tile.rank[j], rows = s_tile.rows[j];
+		const float scale = s_tile.scale[j];
+		float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-			for (int ks = 0; ks < KS; ks++) {
-				const float w0 = c * SP + 2 * ks < rank ? to_float<T>(w[2 * ks]) : 0.0f;
-				const float w1 = c * SP + 2 * ks + 1 < rank ? to_float<T>(w[2 * ks + 1]) : 0.0f;
-				mma_tf32(acc, lo[ks], __float_as_uint(w0), __float_as_uint(w1));
-				mma_tf32(acc, hi[ks], __float_as_uint(w0), __float_as_uint(w1));
-			}
-#pragma unroll
-			for (int e = 0; e < 4; e++)
-				if (rows >> (lane / 4 + 8 * (e >> 1)) & 1)
-					keep[e] = __fmul_rn(scale, acc[e]);
+		for (int ks = 0; ks < KS; ks++) {
+			T w[2];
+			*(uint32_t *)w = now.w[ks];
+			const uint32_t w0 = c * SP + 2 * ks < rank ? __float_as_uint(to_float<T>(w[0])) : 0u;
+			const uint32_t w1 = c * SP + 2 * ks + 1 < rank ? __float_as_uint(to_float<T>(w[1])) : 0u;
+			mma_tf32(low, lo[ks], w0, w1);
+			mma_tf32(acc, hi[ks], w0, w1);
 		}
 #pragma unroll
-		for (int e = 0; e < 4; e++) {
-			const uint32_t r = row0 + lane / 4 + 8 * (e >> 1), n = n0 + c * 2 + (e & 1);
-			if (r < a.m && n < set.n) {
-				const size_t at = (size_t)r * set.n + n;
-				const float base = set.base[at];       // (a row of no adapter keeps its bits)
-				set.y[at] = wants >> (lane / 4 + 8 * (e >> 1)) & 1 ? __fadd_rn(base, keep[e])
-										   : base;
+		for (int h = 0; h < 2; h++) {
+			const uint32_t r = lane / 4 + 8 * h, col = n0 + c * 2;
+			if (!(rows >> r & 1) || col >= set.n)
+				continue;
+			const float v0 = __fadd_rn(now.base[2 * h], __fmul_rn(scale, acc[2 * h] + low[2 * h]));
+			const float v1 = __fadd_rn(now.base[2 * h + 1], __fmul_rn(scale, acc[2 * h + 1] + low[2 * h + 1]));
+			float *y = set.y + (size_t)(row0 + r) * set.n + col;
+			if (pairs) {
+				*(float2 *)y = make_float2(v0, v1);
+			} else {
+				y[0] = v0;
+				if (col + 1 < set.n)
+					y[1] = v1;
 			}
 		}
+		now = next;
+	}
+}
+
+// ---- long batches: 64 rows a CTA -----------------------------------------------------
+//
+// The same two steps where there are rows enough: each of four warps has 16 rows, and the
+// adapter's weights pass through shared memory once for all of them (a prompt's rows
+// share their adapter; where they do not, a warp without rows of an adapter sits
+// it out). 2000 rows, K = N = 4096, rank 64: 28 + 58 us by the kernels above, which
+// read every weight again for each 16 rows.
+constexpr uint32_t ADAPT_LONG_ROWS = 64, ADAPT_STAGES = 3;
+
+__device__ __forceinline__ void cp_async16_zero(void *dst, const void *src, bool ok)
+{
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+		     :: "r"(smem_addr(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+// The distinct adapters of 64 rows, in order; by warp 0. which: the rows' in shared memory.
+__device__ __forceinline__ uint32_t adapt_distinct(const int32_t *which, int32_t *list)
+{
+	const uint32_t lane = threadIdx.x & 31, below = (1u << lane) - 1;
+	const int32_t v0 = which[lane], v1 = which[lane + 32];
+	const uint32_t same0 = __match_any_sync(0xffffffffu, v0), same1 = __match_any_sync(0xffffffffu, v1);
+	const bool f0 = v0 >= 0 && (int)lane == __ffs(same0) - 1;
+	bool f1 = v1 >= 0 && (int)lane == __ffs(same1) - 1;
+	const uint32_t firsts0 = __ballot_sync(0xffffffffu, f0);
+	for (uint32_t left = firsts0; left; left &= left - 1) {
+		const int32_t v = __shfl_sync(0xffffffffu, v0, __ffs(left) - 1);     // (by all lanes)
+		f1 = f1 && v1 != v;
+	}
+	const uint32_t firsts1 = __ballot_sync(0xffffffffu, f1);
+	if (f0)
+		list[__popc(firsts0 & below)] = v0;
+	if (f1)
+		list[__popc(firsts0) + __popc(firsts1 & below)] = v1;
+	return __popc(firsts0) + __popc(firsts1);
+}
+
+template <int RT>
+struct AdaptLong {
+	static constexpr uint32_t A_PITCH = 192;                 // 64 k of a rank; (64 bytes on: other banks)
+	static constexpr uint32_t A_STAGE = RT * A_PITCH;
+	static constexpr uint32_t B_COLS = 64, B_PITCH = RT * 2 + 16;
+	static constexpr uint32_t B_STAGE = B_COLS * B_PITCH;
+};
+
+template <typename T, int RT>
+__global__ void __launch_bounds__(ADAPT_WARPS * 32)
+adapt_shrink_long_kernel(const __grid_constant__ AdaptArgs a)
+{
+	using L = AdaptLong<RT>;
+	constexpr int NT = RT / 8;
+	__shared__ __align__(16) uint8_t s_a[ADAPT_STAGES][L::A_STAGE];
+	__shared__ int32_t s_which[ADAPT_LONG_ROWS], s_list[ADAPT_LONG_ROWS];
+	__shared__ uint32_t s_n;
+	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
+	const uint32_t tile0 = blockIdx.x * ADAPT_LONG_ROWS, row0 = tile0 + warp * ADAPT_ROWS, piece = blockIdx.y;
+	const AdaptSet &set = a.s[blockIdx.z];
+	pdl_wait();
+	pdl_launch_dependents();
+	if (threadIdx.x < ADAPT_LONG_ROWS)
+		s_which[threadIdx.x] = adapt_which(a, set, tile0 + threadIdx.x);
+	__syncthreads();
+	if (warp == 0) {
+		const uint32_t n = adapt_distinct(s_which, s_list);
+		if (lane == 0)
+			s_n = n;
+	}
+	__syncthreads();
+	// the piece in steps of two 32-blocks
+	const uint32_t nb = a.k / 32, steps_all = (nb + 1) / 2, each = (steps_all + a.pieces - 1) / a.pieces;
+	const uint32_t s0 = min(piece * each, steps_all), steps = min(s0 + each, steps_all) - s0;
+	const int32_t mine = s_which[warp * ADAPT_ROWS + (lane & 15)];
+	const int8_t *xq[2];
+	const float *xd[2];
+#pragma unroll
+	for (int h = 0; h < 2; h++) {
+		const uint32_t r = min(row0 + lane / 4 + 8 * h, a.m - 1);     // (rows past the last: not kept)
+		xq[h] = a.q + (size_t)r * a.k + c * 8;
+		xd[h] = a.d + (size_t)r * nb;
+	}
+	float *t = a.t + (((size_t)blockIdx.z * a.pieces + piece) * a.m + row0) * RT;
+	for (uint32_t j = 0; j < s_n; j++) {
+		const int32_t ad = s_list[j];
+		const uint32_t rank = adapt_rank(set, ad);
+		const uint32_t rows = __ballot_sync(0xffffffffu, mine == ad) & 0xffffu;
+		const T *w = (const T *)set.a + (size_t)ad * set.max_rank * a.k;
+		auto fetch = [&](uint32_t s) {
+			// 8 words of 16 bytes a rank
+			for (uint32_t x = threadIdx.x; s < steps && x < RT * 8; x += ADAPT_WARPS * 32) {
+				const uint32_t r = x / 8, k = (s0 + s) * 64 + x % 8 * 8;
+				cp_async16_zero(&s_a[s % ADAPT_STAGES][r * L::A_PITCH + x % 8 * 16],
+						w + (size_t)(r < rank ? r : 0) * a.k + (k < a.k ? k : 0), r < rank && k < a.k);
+			}
+			asm volatile("cp.async.commit_group;" ::: "memory");
+		};
+		float acc[NT][4];
+#pragma unroll
+		for (int n = 0; n < NT; n++)
+			acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+		struct Rows {
+			uint2 x[2][2];        // [block][row]
+			float d[2][2];
+		};
+		auto load = [&](Rows &v, uint32_t s) {
+#pragma unroll
+			for (int b = 0; b < 2; b++)
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					const uint32_t block = (s0 + s) * 2 + b;
+					v.x[b][h] = block < nb ? *(const uint2 *)(xq[h] + block * 32) : make_uint2(0, 0);
+					v.d[b][h] = block < nb ? xd[h][block] : 0.0f;
+				}
+		};
+		__syncthreads();                  // (the last adapter's stages have been read)
+		Rows now, next;
+		for (uint32_t s = 0; s < ADAPT_STAGES - 1; s++)
+			fetch(s);
+		if (rows && steps)
+			load(now, 0);
+		for (uint32_t s = 0; s < steps; s++) {
+			asm volatile("cp.async.wait_group %0;" :: "n"((int)ADAPT_STAGES - 2) : "memory");
+			__syncthreads();
+			fetch(s + ADAPT_STAGES - 1);
+			if (!rows)
+				continue;
+			if (s + 1 < steps)
+				load(next, s + 1);
+			const uint8_t *stage = s_a[s % ADAPT_STAGES];
+#pragma unroll
+			for (int b = 0; b < 2; b++) {
+				uint32_t fa[2][4];
+#pragma unroll
+				for (int x = 0; x < 2; x++) {
+					const uint32_t x0 = x ? now.x[b][0].y : now.x[b][0].x, x1 = x ? now.x[b][1].y : now.x[b][1].x;
+					fa[x][0] = int8_pair<T>(x0, 0);
+					fa[x][1] = int8_pair<T>(x1, 0);
+					fa[x][2] = int8_pair<T>(x0, 2);
+					fa[x][3] = int8_pair<T>(x1, 2);
+				}
+#pragma unroll
+				for (int n = 0; n < NT; n++) {
+					const uint4 v = *(const uint4 *)(stage + (n * 8 + lane / 4) * L::A_PITCH + b * 64 + c * 16);
+					float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+					mma_16816<T>(sum, fa[0], v.x, v.y);
+					mma_16816<T>(sum, fa[1], v.z, v.w);
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						acc[n][e] = __fmaf_rn(now.d[b][e >> 1], sum[e], acc[n][e]);
+				}
+			}
+			now = next;
+		}
+		asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+		for (int n = 0; n < NT; n++)
+#pragma unroll
+			for (int e = 0; e < 4; e += 2)
+				if (rows >> (lane / 4 + 4 * e) & 1)
+					*(float2 *)(t + (lane / 4 + 4 * e) * RT + n * 8 + c * 2) = make_float2(acc[n][e], acc[n][e + 1]);
+	}
+}
+
+// The pieces of t added up, in order, into the first: every CTA of the columns reads them
+__global__ void __launch_bounds__(256)
+adapt_sum_kernel(float4 *t, uint32_t pieces, uint32_t each)
+{
+	pdl_wait();
+	pdl_launch_dependents();
+	const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+	if (i >= each)
+		return;
+	float4 *at = t + (size_t)blockIdx.y * pieces * each + i;
+	float4 v = at[0];
+#pragma unroll 8
+	for (uint32_t p = 1; p < pieces; p++) {
+		const float4 u = at[(size_t)p * each];
+		v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
+	}
+	at[0] = v;
+}
+
+template <typename T, int RT>
+__global__ void __launch_bounds__(ADAPT_WARPS * 32)
+adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
+{
+	using L = AdaptLong<RT>;
+	constexpr int SP = RT / 4, KS = RT / 8;          // ranks a lane; k steps
+	__shared__ __align__(16) uint8_t s_b[ADAPT_STAGES][L::B_STAGE];
+	__shared__ int32_t s_which[ADAPT_LONG_ROWS], s_list[ADAPT_LONG_ROWS];
+	__shared__ uint32_t s_n;
+	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
+	const uint32_t tile0 = blockIdx.x * ADAPT_LONG_ROWS, row0 = tile0 + warp * ADAPT_ROWS;
+	uint32_t si = 0;
+	while (blockIdx.y >= a.s[si].block_end)
+		si++;
+	const AdaptSet &set = a.s[si];
+	const uint32_t col0 = (blockIdx.y - (si ? a.s[si - 1].block_end : 0)) * a.cols;
+	const uint32_t end = min(col0 + a.cols, set.n), steps = (end - col0 + L::B_COLS - 1) / L::B_COLS;
+	const bool fours = set.n % 4 == 0 && !(((uintptr_t)set.base | (uintptr_t)set.y) & 15);
+	pdl_wait();
+	pdl_launch_dependents();
+	if (threadIdx.x < ADAPT_LONG_ROWS)
+		s_which[threadIdx.x] = adapt_which(a, set, tile0 + threadIdx.x);
+	__syncthreads();
+	if (warp == 0) {
+		const uint32_t n = adapt_distinct(s_which, s_list);
+		if (lane == 0)
+			s_n = n;
+	}
+	// this warp's t, straight into the fragments
+	uint32_t hi[KS][4], lo[KS][4];
+#pragma unroll
+	for (int h = 0; h < 2; h++) {
+		const uint32_t r = row0 + lane / 4 + 8 * h;
+		float v[SP];
+#pragma unroll
+		for (int i = 0; i < SP; i++)
+			v[i] = 0.0f;
+		if (r < a.m) {
+			const float *t = a.t + ((size_t)si * a.pieces * a.m + r) * RT + c * SP;
+#pragma unroll
+			for (int i = 0; i < SP; i += SP < 4 ? 2 : 4) {
+				if (SP < 4)
+					*(float2 *)v = *(const float2 *)t;
+				else
+					*(float4 *)(v + i) = *(const float4 *)(t + i);
+			}
+		}
+#pragma unroll
+		for (int i = 0; i < SP; i++) {
+			hi[i / 2][h + 2 * (i % 2)] = __float_as_uint(v[i]) & 0xffffe000u;
+			lo[i / 2][h + 2 * (i % 2)] = __float_as_uint(__fsub_rn(v[i], __uint_as_float(hi[i / 2][h + 2 * (i % 2)])));
+		}
+	}
+	__syncthreads();
+	const int32_t mine = s_which[warp * ADAPT_ROWS + (lane & 15)];
+	const uint32_t wants = __ballot_sync(0xffffffffu, mine >= 0) & 0xffffu;
+	// rows of no adapter keep the base's bits
+	const uint32_t there = row0 >= a.m ? 0 : a.m - row0 < ADAPT_ROWS ? (1u << (a.m - row0)) - 1 : 0xffffu;
+	adapt_copy(set, row0, there & ~wants, col0, end, lane, 32);
+	const uint32_t words = set.max_rank / 8;          // of 16 bytes a column
+	for (uint32_t j = 0; j < s_n; j++) {
+		const int32_t ad = s_list[j];
+		const uint32_t rank = adapt_rank(set, ad);
+		const float scale = set.scale[ad];
+		const uint32_t rows = __ballot_sync(0xffffffffu, mine == ad) & 0xffffu;
+		const T *w = (const T *)set.b + (size_t)ad * set.n * set.max_rank;
+		auto fetch = [&](uint32_t s) {
+			for (uint32_t x = threadIdx.x; s < steps && x < L::B_COLS * words; x += ADAPT_WARPS * 32) {
+				const uint32_t r = x / words, i = x - r * words, n = col0 + s * L::B_COLS + r;
+				cp_async16_zero(&s_b[s % ADAPT_STAGES][r * L::B_PITCH + i * 16],
+						w + (size_t)(n < end ? n : col0) * set.max_rank + i * 8, n < end);
+			}
+			asm volatile("cp.async.commit_group;" ::: "memory");
+		};
+		__syncthreads();                  // (the last adapter's stages have been read)
+		for (uint32_t s = 0; s < ADAPT_STAGES - 1; s++)
+			fetch(s);
+		for (uint32_t s = 0; s < steps; s++) {
+			// Columns are dealt to the MMAs so that a thread has runs of four: column
+			// 16 x + 4 (n / 2) + 2 (g % 2) + n % 2 is the n-th of group g, x = g / 2, so of
+			// groups 2 x and 2 x + 1 thread c has 16 x + 4 c ... + 3. A row's 64 bytes then
+			// move together (not 32, as in the order of the fragments). The bases of this step are on
+			// their way before its weights are waited for.
+			float base[4][2][4];
+			const uint32_t n0 = col0 + s * L::B_COLS + c * 4;
+#pragma unroll
+			for (int x = 0; x < 4; x++)
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					const uint32_t r = lane / 4 + 8 * h, col = n0 + x * 16;
+					const float *b = set.base + (size_t)(row0 + r) * set.n + col;
+					const bool mine_too = rows >> r & 1;
+					float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+					if (fours) {
+						if (mine_too && col < end)
+							v = *(const float4 *)b;
+					} else if (mine_too) {
+						v.x = col < end ? b[0] : 0.0f;
+						v.y = col + 1 < end ? b[1] : 0.0f;
+						v.z = col + 2 < end ? b[2] : 0.0f;
+						v.w = col + 3 < end ? b[3] : 0.0f;
+					}
+					*(float4 *)base[x][h] = v;
+				}
+			asm volatile("cp.async.wait_group %0;" :: "n"((int)ADAPT_STAGES - 2) : "memory");
+			__syncthreads();
+			fetch(s + ADAPT_STAGES - 1);
+			if (!rows)
+				continue;
+			const uint8_t *stage = s_b[s % ADAPT_STAGES];
+#pragma unroll
+			for (int x = 0; x < 4; x++) {
+				float acc[2][4], low[2][4];
+				T wv[2][SP];
+#pragma unroll
+				for (int g = 0; g < 2; g++) {
+					const uint32_t n = lane / 4, col = 16 * x + 4 * (n / 2) + 2 * g + n % 2;
+					const uint8_t *src = stage + col * L::B_PITCH + c * SP * 2;
+#pragma unroll
+					for (int i = 0; i < SP; i += SP < 8 ? SP : 8) {
+						if (SP == 2)
+							*(uint32_t *)wv[g] = *(const uint32_t *)src;
+						else if (SP == 4)
+							*(uint2 *)wv[g] = *(const uint2 *)src;
+						else
+							*(uint4 *)(wv[g] + i) = *(const uint4 *)(src + i * 2);
+					}
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						acc[g][e] = low[g][e] = 0.0f;
+				}
+#pragma unroll
+				for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+					for (int g = 0; g < 2; g++) {
+						const uint32_t w0 = c * SP + 2 * ks < rank ? __float_as_uint(to_float<T>(wv[g][2 * ks])) : 0u;
+						const uint32_t w1 =
+							c * SP + 2 * ks + 1 < rank ? __float_as_uint(to_float<T>(wv[g][2 * ks + 1])) : 0u;
+						mma_tf32(low[g], lo[ks], w0, w1);
+						mma_tf32(acc[g], hi[ks], w0, w1);
+					}
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					const uint32_t r = lane / 4 + 8 * h, col = n0 + x * 16;
+					if (!(rows >> r & 1))
+						continue;
+					float v[4];
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						v[e] = __fadd_rn(base[x][h][e],
+								 __fmul_rn(scale, acc[e / 2][2 * h + e % 2] + low[e / 2][2 * h + e % 2]));
+					float *y = set.y + (size_t)(row0 + r) * set.n + col;
+					if (fours) {
+						if (col < end)
+							*(float4 *)y = make_float4(v[0], v[1], v[2], v[3]);
+					} else {
+#pragma unroll
+						for (int e = 0; e < 4; e++)
+							if (col + e < end)
+								y[e] = v[e];
+					}
+				}
+			}
+		}
+		asm volatile("cp.async.wait_group 0;" ::: "memory");
 	}
 }
 

@@ -318,28 +318,60 @@ uint32_t adapters_ranks(const charsiu_gpu_adapters *s, unsigned n)
 	return most <= 8 ? 8 : most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : 128;
 }
 
-// pieces of K: enough CTAs for two a multiprocessor, at least two 32-blocks a warp
-uint32_t adapters_pieces(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n, unsigned m)
+constexpr uint32_t ADAPT_CTAS_PER_SM = 4, ADAPT_MAX_PIECES = 16, ADAPT_LONG_CTAS_PER_SM = 3;
+constexpr unsigned ADAPT_LONG_M = 256;      // rows from which 64 a CTA fill the GPU
+
+// Whether the rows go 64 to a CTA
+bool adapters_long(const charsiu_gpu_adapters *s, unsigned n, unsigned m)
 {
-	const uint64_t tiles = (uint64_t)n * ((m + ADAPT_ROWS - 1) / ADAPT_ROWS);
-	const uint32_t most = (s->k / 32 + 2 * ADAPT_WARPS - 1) / (2 * ADAPT_WARPS);
-	const uint64_t want = (2ull * layer_sms(g) + tiles - 1) / (tiles ? tiles : 1);
-	return want < 1 ? 1 : want < most ? (uint32_t)want : most;
+	for (unsigned i = 0; i < n; i++)
+		if (s[i].max_rank % 8)          // (weights are copied by 16 bytes)
+			return false;
+	return m >= ADAPT_LONG_M && adapters_ranks(s, n) <= 64;
 }
 
-// scratch for m rows, and for any fewer: pieces * m is at most the CTAs aimed at and
-// a tile's more, in rows
+// pieces of K: enough CTAs to fill the GPU, at least one 32-block a warp
+uint32_t adapters_pieces(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n, unsigned m)
+{
+	const bool lng = adapters_long(s, n, m);
+	const uint64_t rows = lng ? ADAPT_LONG_ROWS : ADAPT_ROWS, tiles = n * ((m + rows - 1) / rows);
+	uint64_t want = (uint64_t)(lng ? ADAPT_LONG_CTAS_PER_SM : ADAPT_CTAS_PER_SM) * layer_sms(g) / (tiles ? tiles : 1);
+	const uint32_t most = (s->k / 32 + ADAPT_WARPS - 1) / ADAPT_WARPS;
+	want = want < most ? want : most;
+	want = want < ADAPT_MAX_PIECES ? want : ADAPT_MAX_PIECES;
+	return want < 1 ? 1 : (uint32_t)want;
+}
+
+// scratch for m rows, and for any fewer: pieces * m is at most the CTAs aimed at and a
+// tile's more, in rows, and at most the most pieces a row
 size_t adapters_bytes(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n, unsigned m)
 {
-	const size_t tiles = (m + ADAPT_ROWS - 1) / ADAPT_ROWS;
-	return (2 * (size_t)layer_sms(g) + n * tiles) * ADAPT_ROWS * adapters_ranks(s, n) * sizeof(float);
+	const size_t rows = ((size_t)m + ADAPT_LONG_ROWS - 1) / ADAPT_LONG_ROWS * ADAPT_LONG_ROWS;
+	const size_t a = ADAPT_MAX_PIECES * rows * n;
+	const size_t b = (size_t)ADAPT_LONG_CTAS_PER_SM * layer_sms(g) * ADAPT_LONG_ROWS + n * rows;
+	return (a < b ? a : b) * adapters_ranks(s, n) * sizeof(float);
 }
 
 template <typename T, int RT>
-int adapters(charsiu_gpu *g, const AdaptArgs &a, void *stream)
+int adapters(charsiu_gpu *g, const AdaptArgs &a, bool lng, void *stream)
 {
+	if constexpr (RT <= 64) {
+		if (lng) {
+			const unsigned tiles = (a.m + ADAPT_LONG_ROWS - 1) / ADAPT_LONG_ROWS;
+			const uint32_t each = a.m * (RT / 4);
+			return launch(g, stream, adapt_shrink_long_kernel<T, RT>, dim3(tiles, a.pieces, a.n_sets),
+				      ADAPT_WARPS * 32, 0, a) &&
+					       (a.pieces == 1 ||
+						launch(g, stream, adapt_sum_kernel, dim3((each + 255) / 256, a.n_sets), 256, 0,
+						       (float4 *)a.t, a.pieces, each)) &&
+					       launch(g, stream, adapt_expand_long_kernel<T, RT>, dim3(tiles, a.blocks),
+						      ADAPT_WARPS * 32, 0, a)
+				       ? 0
+				       : -1;
+		}
+	}
 	const unsigned tiles = (a.m + ADAPT_ROWS - 1) / ADAPT_ROWS;
-	return launch(g, stream, adapt_shrink_kernel<T, RT>, dim3(tiles, a.pieces, a.n_sets),
+	return launch(g, stream, adapt_shrink_kernel<T, RT>, dim3(tiles, a.pieces * a.parts, a.n_sets),
 		      ADAPT_WARPS * 32, 0, a) &&
 			       launch(g, stream, adapt_expand_kernel<T, RT>, dim3(tiles, a.blocks),
 				      ADAPT_WARPS * 32, 0, a)
@@ -348,14 +380,14 @@ int adapters(charsiu_gpu *g, const AdaptArgs &a, void *stream)
 }
 
 template <typename T>
-int adapters_of(charsiu_gpu *g, const AdaptArgs &a, uint32_t ranks, void *stream)
+int adapters_of(charsiu_gpu *g, const AdaptArgs &a, uint32_t ranks, bool lng, void *stream)
 {
 	switch (ranks) {
-	case 8: return adapters<T, 8>(g, a, stream);
-	case 16: return adapters<T, 16>(g, a, stream);
-	case 32: return adapters<T, 32>(g, a, stream);
-	case 64: return adapters<T, 64>(g, a, stream);
-	default: return adapters<T, 128>(g, a, stream);
+	case 8: return adapters<T, 8>(g, a, lng, stream);
+	case 16: return adapters<T, 16>(g, a, lng, stream);
+	case 32: return adapters<T, 32>(g, a, lng, stream);
+	case 64: return adapters<T, 64>(g, a, lng, stream);
+	default: return adapters<T, 128>(g, a, lng, stream);
 	}
 }
 
@@ -381,13 +413,32 @@ int charsiu_gpu_norm_quantise_dev(struct charsiu_gpu *g, const float *x, const f
 	if (!m)
 		return 0;
 	OnDevice on(g);
-	static uint64_t smem_done;
-	if (!allow_smem(g, norm_rows_kernel, norm_rows_smem(NORM_ROWS_MAX_K), smem_done))
-		return -1;
-	return launch(g, stream, norm_rows_kernel, dim3(m), NORM_ROWS_THREADS, norm_rows_smem(k), x, add, w,
-		      (uint32_t)k, eps, x_out, q, d)
-		       ? 0
-		       : -1;
+	// A CTA a row where the rows are few and long: one row of 2048 / 4096 / 8192 takes it
+	// 8.5 / 12.6 / 16.7 us and the chains 10.6 / 18.7 / 35; at 296 rows of 4096 it is
+	// 33 us against 20. The chains: as few rows a CTA (three of them a multiprocessor) as
+	// hold all rows at once: 2048 rows of 4096 take 41 us by 4, 37 by 8, 41 by 16.
+	const uint64_t sms = layer_sms(g), cta = 3;
+	if (k >= 2048 && 4 * (uint64_t)m <= 3 * sms) {
+		static uint64_t smem_done;
+		if (!allow_smem(g, norm_rows_kernel, norm_rows_smem(NORM_ROWS_MAX_K), smem_done))
+			return -1;
+		return launch(g, stream, norm_rows_kernel, dim3(m), NORM_ROWS_THREADS, norm_rows_smem(k), x, add, w,
+			      (uint32_t)k, eps, x_out, q, d)
+			       ? 0
+			       : -1;
+	}
+	auto chains = [&](auto kernel, uint32_t rows, uint64_t &smem_done) {
+		return allow_smem(g, kernel, norm_chain_smem(rows), smem_done) &&
+				       launch(g, stream, kernel, dim3((unsigned)(((uint64_t)m + rows - 1) / rows)),
+					      NORM_CHAIN_THREADS, norm_chain_smem(rows), x, add, w, (uint32_t)m,
+					      (uint32_t)k, eps, x_out, q, d, layer_kernel_error(g))
+			       ? 0
+			       : -1;
+	};
+	static uint64_t done4, done8, done16;
+	return m <= 4 * cta * sms   ? chains(norm_chain_kernel<1>, 4, done4)
+	       : m <= 8 * cta * sms ? chains(norm_chain_kernel<2>, 8, done8)
+				    : chains(norm_chain_kernel<4>, 16, done16);
 }
 
 size_t charsiu_gpu_pages_work(const struct charsiu_gpu_pages *p)
@@ -557,7 +608,8 @@ int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_ada
 	if (!work || misaligned(work, 16) || work_bytes < adapters_bytes(g, sets, n, m))
 		return refuse(g, "adapters: the work array is missing, misaligned or too small");
 	AdaptArgs a = {};
-	uint64_t blocks = 0;
+	uint64_t columns = 0;
+	uint32_t slots = 0;
 	for (unsigned i = 0; i < n; i++) {
 		AdaptSet &s = a.s[i];
 		s.a = sets[i].a;
@@ -571,8 +623,26 @@ int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_ada
 		s.n = sets[i].n;
 		s.slots = sets[i].slots;
 		s.max_rank = sets[i].max_rank;
-		blocks += (s.n + ADAPT_COLS - 1) / ADAPT_COLS;
-		s.block_end = (uint32_t)blocks;
+		columns += s.n;
+		slots = slots > s.slots ? slots : s.slots;
+	}
+	// CTAs over the columns: as wide as still fills the GPU
+	const bool lng = adapters_long(sets, n, m);
+	const uint64_t tile = lng ? ADAPT_LONG_ROWS : ADAPT_ROWS, tiles = (m + tile - 1) / tile;
+	const uint64_t aim = (uint64_t)(lng ? ADAPT_LONG_CTAS_PER_SM : ADAPT_CTAS_PER_SM) * layer_sms(g);
+	if (lng) {
+		// (narrower than fills it: a tile of several adapters takes as many times as long)
+		a.cols = (uint32_t)((tiles * columns / (2 * aim) + 63) / 64 * 64);
+		a.cols = a.cols < 64 ? 64 : a.cols > 512 ? 512 : a.cols;
+	} else {
+		a.cols = 256;
+		while (a.cols > 32 && tiles * columns / a.cols < aim)
+			a.cols /= 2;
+	}
+	uint64_t blocks = 0;
+	for (unsigned i = 0; i < n; i++) {
+		blocks += (a.s[i].n + a.cols - 1) / a.cols;
+		a.s[i].block_end = (uint32_t)blocks;
 	}
 	if (blocks > 65535)
 		return refuse(g, "adapters: more columns than a call takes");
@@ -584,11 +654,17 @@ int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_ada
 	a.m = m;
 	a.k = sets[0].k;
 	a.pieces = adapters_pieces(g, sets, n, m);
+	// few tiles: their distinct adapters over several CTAs, as far as the GPU has room
+	uint64_t parts = aim / (tiles * n * a.pieces);
+	parts = parts < ADAPT_ROWS ? parts : ADAPT_ROWS;
+	parts = parts < slots ? parts : slots;
+	parts = parts < m ? parts : m;
+	a.parts = parts < 1 ? 1 : (uint32_t)parts;
 	a.blocks = (uint32_t)blocks;
 	OnDevice on(g);
 	const uint32_t ranks = adapters_ranks(sets, n);
-	return sets[0].type == TYPE_F16 ? adapters_of<__half>(g, a, ranks, stream)
-					: adapters_of<__nv_bfloat16>(g, a, ranks, stream);
+	return sets[0].type == TYPE_F16 ? adapters_of<__half>(g, a, ranks, lng, stream)
+					: adapters_of<__nv_bfloat16>(g, a, ranks, lng, stream);
 }
 
 } // extern "C"
