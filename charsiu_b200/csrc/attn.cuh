@@ -45,6 +45,7 @@ struct AttnArgs {
 	uint32_t rows_splits;                 // pieces of the prefix that the rows kernel makes
 	uint32_t out_type;
 	uint32_t behind;      // the rows kernel: behind the prefix's launch, no wait for it
+	uint32_t early;       // and its CTAs that fit beside that launch's
 	float scale;          // scale * log2(e)
 	int *err;             // a wait that gave up says so here
 };
@@ -132,10 +133,14 @@ __device__ __forceinline__ AttnGroup attn_group_of(const AttnArgs &a, uint32_t s
 	return r;
 }
 
-// Unit u of all groups' row tiles (`rows` rows each): its group and the tile in
-// it; false past the last. By a whole warp.
-__device__ __forceinline__ bool attn_find_unit(const AttnArgs &a, uint32_t u, uint32_t rows,
-					       AttnGroup *g, uint32_t *tile)
+// Unit u of all groups' row tiles (`rows` rows each): its group's bounds and told shared
+// pages, and the tile in it; false past the last. By a whole warp.
+struct AttnUnit {
+	int32_t b0, b1, told;
+	uint32_t tile;
+};
+
+__device__ __forceinline__ bool attn_find_unit(const AttnArgs &a, uint32_t u, uint32_t rows, AttnUnit *at)
 {
 	const uint32_t lane = threadIdx.x & 31;
 	uint32_t before = 0;
@@ -156,9 +161,10 @@ __device__ __forceinline__ bool attn_find_unit(const AttnArgs &a, uint32_t u, ui
 		const uint32_t who = __ballot_sync(0xffffffffu, u >= lo && u < lo + n);
 		if (who) {
 			const int src = __ffs(who) - 1;
-			*tile = u - __shfl_sync(0xffffffffu, lo, src);
-			*g = attn_group(a, __shfl_sync(0xffffffffu, b0, src), __shfl_sync(0xffffffffu, b1, src),
-					__shfl_sync(0xffffffffu, told, src));
+			at->tile = u - __shfl_sync(0xffffffffu, lo, src);
+			at->b0 = __shfl_sync(0xffffffffu, b0, src);
+			at->b1 = __shfl_sync(0xffffffffu, b1, src);
+			at->told = __shfl_sync(0xffffffffu, told, src);
 			return true;
 		}
 		before += __shfl_sync(0xffffffffu, inc, 31);
@@ -284,6 +290,52 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, int x
 }
 
 constexpr int ATTN_THREADS = (ATTN_WARPS + 1) * 32;
+
+// How many CTAs of the rows kernel take items. Beside the prefix's launch the first a.early of
+// them start with it, the others when its CTAs end: where the sequences' own keys are
+// little work, the first take it all while the prefix is computed. The estimate is in
+// microseconds: a stage of keys takes a CTA 0.8, an item 2 more, the prefix's steps of 64
+// keys 0.9 each and 10 around them. Every CTA comes to the same answer. By a whole warp.
+template <int HD>
+__device__ __forceinline__ uint32_t attn_takers(const AttnArgs &a)
+{
+	const uint32_t lane = threadIdx.x & 31;
+	if (!a.behind || a.early >= gridDim.x || a.n_seq > 128 || a.n_group > 32)
+		return gridDim.x;
+	const bool real = lane < a.n_group;
+	const int32_t b0 = real ? __ldcg(&a.group[lane]) : 0, b1 = real ? __ldcg(&a.group[lane + 1]) : 0;
+	const int32_t told = real ? __ldcg(&a.shared[lane]) : 0;
+	int32_t slot[4], own[4];
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		slot[j] = lane + 32 * j < a.n_seq ? __ldcg(&a.slots[lane + 32 * j]) : -1;
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		own[j] = attn_slot_len(a, slot[j]);
+	float keys = 0.0f, longest = 0.0f;
+	for (uint32_t g = 0; g < a.n_group; g++) {
+		const int32_t c0 = __shfl_sync(0xffffffffu, b0, g), c1 = __shfl_sync(0xffffffffu, b1, g);
+		const int32_t pages = min(__shfl_sync(0xffffffffu, told, g), (int32_t)a.p.max_pages);
+		const int32_t shared = max(pages, 0) * (int32_t)a.p.page;
+		longest = fmaxf(longest, (float)shared);
+#pragma unroll
+		for (int j = 0; j < 4; j++) {
+			const int32_t s = (int32_t)lane + 32 * j;
+			if (s >= c0 && s < c1)
+				own[j] = max(own[j] - shared, 0);
+		}
+	}
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		keys += (float)own[j];
+	for (int o = 16; o; o >>= 1)
+		keys += __shfl_xor_sync(0xffffffffu, keys, o);
+	const float items = (float)a.own_tiles * a.p.n_head_kv;
+	const float t_own = items * (0.8f * keys / AttnRing<HD>::KEYS + 2.0f * a.n_seq) / a.early;
+	const float t_prefix = 10.0f + 0.9f * longest / 64.0f / (a.pre_splits / 2);
+	return t_own <= 1.2f * t_prefix ? a.early : gridDim.x;
+}
+
 // codes of a wait that gave up, after the batched matvec's (5 to 13)
 constexpr int ATTN_ERR_RING = 24, ATTN_ERR_ROWS = 25;
 
@@ -299,7 +351,8 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 	__shared__ __align__(8) uint64_t b_full[NS], b_free[NS];
 	__shared__ __align__(8) uint64_t b_join;
 	__shared__ AttnStage s_stage[NS];
-	__shared__ float s_m[ATTN_WARPS][ATTN_TILE_ROWS], s_l[ATTN_WARPS][ATTN_TILE_ROWS];
+	// (two items' maxima and sums: one warp may be at the next while another reads the last's)
+	__shared__ float s_m[2][ATTN_WARPS][ATTN_TILE_ROWS], s_l[2][ATTN_WARPS][ATTN_TILE_ROWS];
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 	const uint32_t ring = smem_addr(rows_raw);
 	uint8_t *ring_ptr = rows_raw;
@@ -318,7 +371,6 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 	// one does not touch. It ends after that one, as the join counts on.
 	if (!a.behind)
 		pdl_wait();
-	pdl_launch_dependents();
 	const uint32_t pre_items = a.pre_units * kvh_n * a.rows_splits;
 	const uint32_t own_items = a.n_seq * a.own_tiles * kvh_n * a.own_splits, items = pre_items + own_items;
 
@@ -365,9 +417,10 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 			__syncwarp();
 			c++;
 		};
+		const uint32_t ctas = attn_takers<HD>(a);
 		// a lane an item, 32 items' lengths and groups on their way at a time
-		for (uint64_t at = blockIdx.x; at < items && ok; at += 32ull * gridDim.x) {
-			const uint64_t it = at + (uint64_t)lane * gridDim.x;
+		for (uint64_t at = blockIdx.x < ctas ? blockIdx.x : items; at < items && ok; at += 32ull * ctas) {
+			const uint64_t it = at + (uint64_t)lane * ctas;
 			const bool own = it >= pre_items && it < items;
 			const uint32_t splits = own ? a.own_splits : max(a.rows_splits, 1u);
 			uint32_t b = own ? (uint32_t)(it - pre_items) : (uint32_t)min(it, (uint64_t)items);
@@ -423,9 +476,13 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 				int32_t from = __shfl_sync(0xffffffffu, k0, j), of = __shfl_sync(0xffffffffu, slot, j);
 				if (what & 16) {
 					// a prefix's unit
-					AttnGroup gr;
-					if (!attn_find_unit(a, g.s0, ATTN_TILE_ROWS, &gr, &g.tile) || !gr.keys)
+					AttnUnit at;
+					if (!attn_find_unit(a, g.s0, ATTN_TILE_ROWS, &at))
 						continue;
+					const AttnGroup gr = attn_group(a, at.b0, at.b1, at.told);
+					if (!gr.keys)
+						continue;
+					g.tile = at.tile;
 					g.s0 = gr.s0;
 					g.n_rows = (gr.s1 - gr.s0) * tg;
 					g.len = 0x7fffffff;
@@ -506,8 +563,10 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 #pragma unroll
 				for (int e = 0; e < 2; e++) {
 					const uint32_t r = h.tile * ATTN_TILE_ROWS + lane / 4 + 8 * e;
-					limit[e] = r < h.n_rows ? h.len - (int32_t)a.n_tok + (int32_t)(r % tg / a.gqa) + 1
-								: h.k1;
+					// (a prefix is seen whole)
+					limit[e] = r < h.n_rows && !(h.kind & 16)
+							   ? h.len - (int32_t)a.n_tok + (int32_t)(r / a.gqa) + 1
+							   : h.k1;
 				}
 				least = min(min(__reduce_min_sync(0xffffffffu, limit[0]),
 						__reduce_min_sync(0xffffffffu, limit[1])), h.k1);
@@ -664,15 +723,15 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 			}
 			if (h.kind & 2) {
 				// the warps joined: maxima and sums, then the outputs through this stage
-				const uint32_t row0 = h.tile * ATTN_TILE_ROWS;
+				const uint32_t row0 = h.tile * ATTN_TILE_ROWS, turn = joins / 2 & 1;
 				const uint32_t rows = min(h.n_rows - row0, ATTN_TILE_ROWS);
 #pragma unroll
 				for (int e = 0; e < 2; e++) {
 					l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
 					l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
 					if (q4 == 0) {
-						s_m[warp][lane / 4 + 8 * e] = m[e];
-						s_l[warp][lane / 4 + 8 * e] = l[e];
+						s_m[turn][warp][lane / 4 + 8 * e] = m[e];
+						s_l[turn][warp][lane / 4 + 8 * e] = l[e];
 					}
 				}
 				if (!together())                           // all have read the stage
@@ -690,20 +749,21 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 					break;
 				for (uint32_t x = threadIdx.x; x < rows * (HD / 4); x += ATTN_WARPS * 32) {
 					const uint32_t r = x / (HD / 4), i = x % (HD / 4) * 4, rr = row0 + r;
-					if ((h.kind & 16) && !attn_len(a, h.s0 + rr / tg))
+					const uint32_t ss = h.kind & 16 ? rr / tg : 0, in = rr - ss * tg, tok = in / a.gqa;
+					if ((h.kind & 16) && !attn_len(a, h.s0 + ss))
 						continue;              // (its own pieces say that it sees nothing)
 					float top = -INFINITY, sum = 0.0f, f[ATTN_WARPS];
 #pragma unroll
 					for (int w = 0; w < (int)ATTN_WARPS; w++)
-						top = fmaxf(top, s_m[w][r]);
+						top = fmaxf(top, s_m[turn][w][r]);
 					const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
 					for (int w = 0; w < (int)ATTN_WARPS; w++) {
-						f[w] = exp2_approx(s_m[w][r] - base);
-						sum += f[w] * s_l[w][r];
+						f[w] = exp2_approx(s_m[turn][w][r] - base);
+						sum += f[w] * s_l[turn][w][r];
 					}
-					const size_t at = ((size_t)((h.s0 + rr / tg) * a.n_tok + rr % tg / a.gqa) * a.n_head +
-							   h.kvh * a.gqa + rr % a.gqa) * pieces;
+					const size_t at = ((size_t)((h.s0 + ss) * a.n_tok + tok) * a.n_head + h.kvh * a.gqa +
+							   in - tok * a.gqa) * pieces;
 					const float inv = sum != 0.0f ? __fdiv_rn(1.0f, sum) : 0.0f;
 					if (i == 0)
 						a.part_w[at + h.slot_at] = sum != 0.0f ? base + log2f(sum) : -INFINITY;
@@ -721,8 +781,6 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 						make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
 				}
 				fence_proxy_async_smem();
-				if (!together())                           // (s_m and s_l are free again)
-					break;
 			}
 			__syncwarp();
 			if (lane == 0)
@@ -731,6 +789,9 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 		if (!ended && lane == 0)
 			*(volatile int *)a.err = ATTN_ERR_ROWS;
 	}
+	// (Only now: the join's CTAs, waiting beside this kernel from its start, took 64 x 16384
+	// keys from 41 to 53 us.)
+	pdl_launch_dependents();
 	if (a.behind)
 		pdl_wait();
 }
@@ -741,7 +802,6 @@ __global__ void __launch_bounds__(256)
 attn_join_kernel(const __grid_constant__ AttnArgs a)
 {
 	pdl_wait();
-	pdl_launch_dependents();
 	const uint32_t lane = threadIdx.x & 31;
 	const size_t row = (size_t)blockIdx.x * 8 + threadIdx.x / 32;
 	if (row >= (size_t)a.n_seq * a.n_tok * a.n_head)

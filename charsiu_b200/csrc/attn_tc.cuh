@@ -162,7 +162,20 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 	const uint32_t q_at = smem_addr(atc_raw);
 	uint8_t *q_ptr = atc_raw;
 
-	// barriers and tensor memory while the kernel before is still running
+	pdl_wait();
+	pdl_launch_dependents();
+
+	// which rows, which keys (every warp for itself). The launch has room for more units
+	// than there may be (each group can end in a part of one): those leave at once.
+	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa, splits = a.pre_splits / 2;
+	uint32_t b = blockIdx.x;
+	const uint32_t u = b / (kvh_n * splits);
+	b -= u * kvh_n * splits;
+	const uint32_t piece = b / kvh_n, kvh = b - piece * kvh_n;
+	AttnUnit unit;
+	if (!attn_find_unit(a, u, ATC_ROWS, &unit))
+		return;
+	const uint32_t tile = unit.tile;
 	if (warp == 8) {
 		if (lane == 0) {
 			for (uint32_t i = 0; i <= NB; i++) {
@@ -184,18 +197,7 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 		tmem_alloc(&s_tmem, 512);
 		tmem_relinquish();
 	}
-	pdl_wait();
-	pdl_launch_dependents();
-
-	// which rows, which keys (every warp for itself)
-	const uint32_t kvh_n = a.p.n_head_kv, tg = a.n_tok * a.gqa, splits = a.pre_splits / 2;
-	uint32_t b = blockIdx.x;
-	const uint32_t u = b / (kvh_n * splits);
-	b -= u * kvh_n * splits;
-	const uint32_t piece = b / kvh_n, kvh = b - piece * kvh_n;
-	uint32_t tile = 0;
-	AttnGroup gr = {0, 0, 0, -1};
-	attn_find_unit(a, u, ATC_ROWS, &gr, &tile);
+	const AttnGroup gr = attn_group(a, unit.b0, unit.b1, unit.told);
 	int32_t k0 = 0, k1 = gr.keys;
 	attn_piece(k0, k1, piece, splits, ATC_KEYS);
 	const uint32_t n_rows = (gr.s1 - gr.s0) * tg, row0 = tile * ATC_ROWS;

@@ -209,12 +209,15 @@ bool attention_plan(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gp
 		return false;
 	const bool tc = all >= 32;
 	const uint32_t unit = tc ? ATC_ROWS : ATTN_TILE_ROWS;
-	a->pre_units = (uint32_t)((all + unit - 1) / unit);
-	a->pre_splits = tc ? 2 * splits((uint64_t)a->pre_units * p->n_head_kv, sms, b->max_len / ATC_KEYS + 1)
-			   : splits((uint64_t)a->pre_units * p->n_head_kv, ATTN_CTAS_PER_SM * sms,
+	const uint32_t units = (uint32_t)((all + unit - 1) / unit);
+	// (three eighths of the multiprocessors are left to the rows kernel beside it: 48 queries of
+	// 4 on 3 x 3000 keys of hd 64 take 37 us with the prefix on all and the rest after it,
+	// 34 with a quarter left, 28 with three eighths; 64 on 16384 of hd 128 55, 58, 51)
+	a->pre_splits = tc ? 2 * splits((uint64_t)units * p->n_head_kv, sms * 5 / 8, b->max_len / ATC_KEYS + 1)
+			   : splits((uint64_t)units * p->n_head_kv, ATTN_CTAS_PER_SM * sms,
 				    b->max_len / ATTN_GRAIN + 1);
 	a->rows_splits = tc ? 0 : a->pre_splits;
-	a->pre_units += b->n_group;          // each group may end in a part of a unit
+	a->pre_units = (uint32_t)((all + (uint64_t)b->n_group * (unit - 1)) / unit);     // each group may end in a part of one
 	return tc;
 }
 
@@ -258,20 +261,26 @@ bool attention_map(CUtensorMap *map, const charsiu_gpu_pages *p, const void *bas
 template <typename T, int HD>
 int attention(charsiu_gpu *g, AttnArgs &a, bool tc, void *stream)
 {
-	static uint64_t smem_done, tc_done;
+	static uint64_t smem_done, tc_done, join_done;
 	CUtensorMap kmap, vmap;
 	if (!attention_map(&kmap, &a.p, a.p.k, a.layer) || !attention_map(&vmap, &a.p, a.p.v, a.layer))
 		return refuse(g, "the cache's strides cannot be described to the copy engine");
 	if (!allow_smem(g, attn_rows_kernel<T, HD>, AttnRing<HD>::SMEM, smem_done) ||
-	    !allow_smem(g, attn_tc_kernel<T, HD>, atc_smem<HD>(), tc_done))
+	    !allow_smem(g, attn_tc_kernel<T, HD>, atc_smem<HD>(), tc_done) ||
+	    !allow_smem(g, attn_join_kernel<T, HD>, 0, join_done))
 		return -1;
 	if (tc && !launch(g, stream, attn_tc_kernel<T, HD>,
 			  dim3(a.pre_units * a.p.n_head_kv * (a.pre_splits / 2)), ATC_THREADS, atc_smem<HD>(), a,
 			  kmap, vmap))
 		return -1;
 	if (tc) {
+		// (without the room for groups' ends, whose CTAs leave at once)
+		const uint64_t busy = (((uint64_t)a.n_seq * a.n_tok * a.gqa + ATC_ROWS - 1) / ATC_ROWS) *
+				      a.p.n_head_kv * (a.pre_splits / 2);
+		const uint64_t sms = layer_sms(g);
 		a.pre_units = 0;
 		a.behind = 1;
+		a.early = busy + 8 <= sms ? (uint32_t)(ATTN_CTAS_PER_SM * (sms - busy)) : 0xffffffffu;
 	}
 	const uint64_t items = (uint64_t)a.p.n_head_kv * ((uint64_t)a.pre_units * a.rows_splits +
 							  (uint64_t)a.n_seq * a.own_tiles * a.own_splits);
@@ -319,9 +328,12 @@ uint32_t adapters_ranks(const charsiu_gpu_adapters *s, unsigned n)
 }
 
 constexpr uint32_t ADAPT_CTAS_PER_SM = 4, ADAPT_MAX_PIECES = 16, ADAPT_LONG_CTAS_PER_SM = 3;
-constexpr unsigned ADAPT_LONG_M = 256;      // rows from which 64 a CTA fill the GPU
+constexpr unsigned ADAPT_LONG_M = 512;
 
-// Whether the rows go 64 to a CTA
+// Whether the rows go 64 to a CTA. Measured, K = N = 4096, 16 rows a CTA against 64: 256 rows of
+// rank 16 13 against 20 us, of rank 64 35 against 34; 512 rows 18 against 18, and 46 against 34;
+// 1000 rows 31 against 27, and 56 against 42. With the rows' adapters mixed, 256 rows 32 against
+// 40 us, 1000 rows 99 against 76.
 bool adapters_long(const charsiu_gpu_adapters *s, unsigned n, unsigned m)
 {
 	for (unsigned i = 0; i < n; i++)

@@ -645,8 +645,8 @@ def check_adapters(q, d, which, mats, ranks, scale, bases, ys):
     (1, 32, [1], 1, 4, BF16), (1, 2048, [2048, 512, 512], 4, 16, BF16), (3, 96, [7, 130], 2, 8, F16),
     (16, 1024, [129], 16, 24, F16), (17, 512, [64, 1], 3, 64, BF16), (33, 2048, [300], 40, 32, BF16),
     (70, 256, [1000], 2, 128, F16), (40, 128, [33], 5, 104, BF16), (600, 160, [96], 3, 40, F16),
-    (5, 14336, [48], 5, 16, BF16), (300, 992, [130, 7], 70, 16, BF16), (257, 64, [64], 1, 8, F16),
-    (333, 320, [201, 66], 4, 64, BF16), (290, 32, [40], 3, 4, F16)])
+    (5, 14336, [48], 5, 16, BF16), (560, 992, [130, 7], 70, 16, BF16), (513, 64, [64], 1, 8, F16),
+    (530, 320, [201, 66], 4, 64, BF16), (520, 32, [40], 3, 4, F16), (515, 96, [68], 2, 128, BF16)])
 def test_adapters(layer, m, k, ns, slots, max_rank, ty):
     rng = np.random.default_rng(m + k)
     mats, ranks, scale = make_adapters(rng, slots, max_rank, k, ns, ty)
