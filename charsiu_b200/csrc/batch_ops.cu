@@ -1,13 +1,15 @@
 // SPDX-License-Identifier: GPL-2.0-or-later
 // The operators of a batched step: argument checks, launch shapes and the C entry
 // points of include/charsiu_gpu.h. The kernels are in norm_rows.cuh, pages.cuh,
-// attn.cuh and adapters.cuh.
+// attn.cuh, attn_tc.cuh and adapters.cuh.
 //
 // Every launch has the programmatic attribute, and every kernel waits for its
-// predecessor before it reads or writes anything of the caller's.
+// predecessor before it reads or writes anything of the caller's (one, behind a launch
+// of its own call, waits at its end: attn_rows_kernel).
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>          // PFN_cuTensorMapEncodeTiled
 
+#include <atomic>
 #include <cstdio>
 #include <type_traits>
 
@@ -83,7 +85,7 @@ bool launch(charsiu_gpu *g, void *stream, K kernel, dim3 grid, unsigned block, s
 // more than 48 KB of shared memory, asked for once a kernel and device; and the whole of a
 // multiprocessor's as shared memory, so that CTAs of different kernels find room on one
 template <typename K>
-bool allow_smem(charsiu_gpu *g, K kernel, size_t bytes, uint64_t &done)
+bool allow_smem(charsiu_gpu *g, K kernel, size_t bytes, std::atomic<uint64_t> &done)
 {
 	const uint64_t bit = 1ull << (layer_device(g) & 63);
 	if (done & bit)
@@ -261,7 +263,7 @@ bool attention_map(CUtensorMap *map, const charsiu_gpu_pages *p, const void *bas
 template <typename T, int HD>
 int attention(charsiu_gpu *g, AttnArgs &a, bool tc, void *stream)
 {
-	static uint64_t smem_done, tc_done, join_done;
+	static std::atomic<uint64_t> smem_done, tc_done, join_done;
 	CUtensorMap kmap, vmap;
 	if (!attention_map(&kmap, &a.p, a.p.k, a.layer) || !attention_map(&vmap, &a.p, a.p.v, a.layer))
 		return refuse(g, "the cache's strides cannot be described to the copy engine");
@@ -431,7 +433,7 @@ int charsiu_gpu_norm_quantise_dev(struct charsiu_gpu *g, const float *x, const f
 	// hold all rows at once: 2048 rows of 4096 take 41 us by 4, 37 by 8, 41 by 16.
 	const uint64_t sms = layer_sms(g), cta = 3;
 	if (k >= 2048 && 4 * (uint64_t)m <= 3 * sms) {
-		static uint64_t smem_done;
+		static std::atomic<uint64_t> smem_done;
 		if (!allow_smem(g, norm_rows_kernel, norm_rows_smem(NORM_ROWS_MAX_K), smem_done))
 			return -1;
 		return launch(g, stream, norm_rows_kernel, dim3(m), NORM_ROWS_THREADS, norm_rows_smem(k), x, add, w,
@@ -439,7 +441,7 @@ int charsiu_gpu_norm_quantise_dev(struct charsiu_gpu *g, const float *x, const f
 			       ? 0
 			       : -1;
 	}
-	auto chains = [&](auto kernel, uint32_t rows, uint64_t &smem_done) {
+	auto chains = [&](auto kernel, uint32_t rows, std::atomic<uint64_t> &smem_done) {
 		return allow_smem(g, kernel, norm_chain_smem(rows), smem_done) &&
 				       launch(g, stream, kernel, dim3((unsigned)(((uint64_t)m + rows - 1) / rows)),
 					      NORM_CHAIN_THREADS, norm_chain_smem(rows), x, add, w, (uint32_t)m,
@@ -447,7 +449,7 @@ int charsiu_gpu_norm_quantise_dev(struct charsiu_gpu *g, const float *x, const f
 			       ? 0
 			       : -1;
 	};
-	static uint64_t done4, done8, done16;
+	static std::atomic<uint64_t> done4, done8, done16;
 	return m <= 4 * cta * sms   ? chains(norm_chain_kernel<1>, 4, done4)
 	       : m <= 8 * cta * sms ? chains(norm_chain_kernel<2>, 8, done8)
 				    : chains(norm_chain_kernel<4>, 16, done16);

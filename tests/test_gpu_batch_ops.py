@@ -539,6 +539,128 @@ def test_attention_takes_nothing_from_behind(layer, value, t):
             assert torch.isnan(got[:, t - 1]).all() or value == -float("inf")
 
 
+def test_attention_of_many_groups_and_sequences(layer):
+    """More sequences than the rows kernel's estimate looks at, more groups than a warp has lanes, pads and
+    empty sequences inside the groups, a scale below 0."""
+    rng = np.random.default_rng(31)
+    for groups, each, t, heads, scale in ((40, 4, 1, 8, None), (3, 50, 2, 4, -0.07), (1, 140, 1, 8, -0.2)):
+        sizes = [[int(v) for v in rng.integers(t, 60, each)] for _ in range(groups)]
+        for g in sizes:
+            g[1] = t                       # as short as can be
+        shared = [int(v) for v in rng.integers(0, 12, groups)]
+        c, slots, bounds, lens, table = build_batch(layer, rng, sizes, shared, t, heads, 2, 64, 16, BF16)
+        for g in range(groups):            # a pad and an emptied sequence in each group
+            slots[bounds[g]] = -1 if g % 2 else len(lens) + 5
+            lens[slots[bounds[g] + 2]] = 0
+        c.len.copy_(torch.from_numpy(lens))
+        q = queries(rng, len(slots) * t, heads, 64, BF16)
+        q.view(len(slots), t, heads, 64)[bounds[0]] = float("nan")        # (what a pad holds)
+        out = run_attention(layer, c, slots, bounds, shared, t, heads, q, scale=scale)
+        known = [s if s < len(lens) else -1 for s in slots]
+        check_attention(c, known, lens, table, t, heads, q, out, scale=scale)
+
+
+def test_attention_of_a_whole_prompt(layer):
+    """As many queries as positions, causal: the rows of a prompt, and of one that goes on from shared pages."""
+    rng = np.random.default_rng(32)
+    for n_tok, sizes, shared in ((90, [[90, 130, 200]], [0]), (60, [[60, 75]], [5])):
+        c, slots, bounds, lens, table = build_batch(layer, rng, sizes, shared, n_tok, 4, 2, 64, 32, F16)
+        q = queries(rng, len(slots) * n_tok, 4, 64, F16)
+        out = run_attention(layer, c, slots, bounds, shared, n_tok, 4, q)
+        check_attention(c, slots, lens, table, n_tok, 4, q, out)
+
+
+def test_attention_goes_by_the_lengths_of_the_replay(layer):
+    """One captured call, replayed as the sequences, their groups and their shared pages change."""
+    rng = np.random.default_rng(33)
+    c, slots, bounds, lens, table = build_batch(layer, rng, [[40] * 9], [14], 1, 16, 2, 128, 16, BF16, spare=20)
+    q = queries(rng, 9, 16, 128, BF16)
+    out = torch.empty_like(q)
+    sl, gr, sh = c.ints(slots), c.ints(bounds), c.ints([14])
+    b = AttentionStruct(slots=sl.data_ptr(), group=gr.data_ptr(), shared=sh.data_ptr(), n_seq=9, n_tok=1, n_head=16,
+                        n_group=1, max_len=300, out_type=BF16, scale=128 ** -0.5)
+    w = scratch(layer.attention_work(c.p, b))
+    b.work, b.work_bytes = w.data_ptr(), w.numel()
+    side = torch.cuda.Stream()
+    layer.attention_dev(c.p, 1, b, q.data_ptr(), out.data_ptr(), side.cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        layer.attention_dev(c.p, 1, b, q.data_ptr(), out.data_ptr(), side.cuda_stream)
+    for told, cut in ((14, [40] * 9), (3, [40, 1, 17, 0, 40, 33, 2, 9, 16]), (0, [0] * 9), (14, [16, 40, 40, 40, 0, 8, 8, 8, 1])):
+        for s, own in zip(slots, cut):
+            lens[s] = 14 * 16 + own if own else (14 * 16 if told == 14 else 0)
+        c.len.copy_(torch.from_numpy(lens))
+        sh.fill_(told)
+        q.copy_(queries(rng, 9, 16, 128, BF16))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(c, slots, lens, table, 1, 16, q, out)
+
+
+def test_calls_on_two_streams_at_once(layer):
+    """Attention and adapters on two streams, each with scratch of its own, many times over: the results of the
+    calls alone."""
+    rng = np.random.default_rng(34)
+    jobs = []
+    for hd, n in ((64, 24), (128, 12)):
+        c, slots, bounds, lens, table = build_batch(layer, rng, [[30] * n], [40], 1, 16, 2, hd, 16, BF16)
+        q = queries(rng, n, 16, hd, BF16)
+        want = run_attention(layer, c, slots, bounds, [40], 1, 16, q)
+        out = torch.empty_like(q)
+        keep = [c.ints(slots), c.ints(bounds), c.ints([40])]
+        b = AttentionStruct(slots=keep[0].data_ptr(), group=keep[1].data_ptr(), shared=keep[2].data_ptr(), n_seq=n, n_tok=1,
+                            n_head=16, n_group=1, max_len=700, out_type=BF16, scale=hd ** -0.5)
+        w = scratch(layer.attention_work(c.p, b))
+        b.work, b.work_bytes = w.data_ptr(), w.numel()
+        jobs.append((torch.cuda.Stream(), c, b, q, out, want.view_as(out), w, keep))
+    torch.cuda.synchronize()
+    for _ in range(40):
+        for st_, c, b, q, out, *_ in jobs:
+            layer.attention_dev(c.p, 1, b, q.data_ptr(), out.data_ptr(), st_.cuda_stream)
+    torch.cuda.synchronize()
+    for _, _, _, _, out, want, *_ in jobs:
+        assert torch.equal(out, want)
+
+
+def test_offsets_past_32_bits(layer):
+    """A cache whose second layer lies past 2^32 elements: append, fork and attention there."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    rng = np.random.default_rng(35)
+    c, slots, bounds, lens, table = build_batch(layer, rng, [[9, 20, 33]], [3], 1, 4, 2, 64, 16, BF16, layers=1)
+    far = (1 << 32) + 4096
+    need = far + c.k.numel()
+    big = [torch.empty(need, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for x, pool in zip(big, (c.k, c.v)):
+        x[:pool.numel()] = float("nan")
+        x[far:] = pool.flatten()
+    c.p.k, c.p.v, c.p.n_layer, c.p.layer_stride = big[0].data_ptr(), big[1].data_ptr(), 2, far
+    c.k, c.v = [torch.stack((x[:pool.numel()].view(pool.shape[1:]), x[far:].view(pool.shape[1:]))) for x, pool in zip(big, (c.k, c.v))]
+    q = queries(rng, 3, 4, 64, BF16)
+    out = run_attention(layer, c, slots, bounds, [3], 1, 4, q, at=1)
+    check_attention(c, slots, lens, table, 1, 4, q, out, at=1)
+    # append one row to layer 1, fork it, and see both through the pool
+    xs = [dev(rng.standard_normal((1, h * 64)).astype(np.float32)) for h in (4, 2, 2)]
+    cs, q_out, sl = dev(rope_table(256, 64)), torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda"), c.ints([slots[0]])
+    layer.pages_append_dev(c.p, 1, sl.data_ptr(), 1, 1, 4, *[x.data_ptr() for x in xs], cs.data_ptr(), 256, q_out.data_ptr(), st())
+    ref = torch.zeros(c.p.n_pages, dtype=torch.int32)
+    for s in slots:
+        for j in range(-(-int(lens[s]) // 16)):
+            ref[table[s, j]] += 1
+    c.ref.copy_(ref)
+    empty = next(s for s in range(len(lens)) if s not in slots)
+    c.fork([slots[0]], [empty])
+    torch.cuda.synchronize()
+    pos = int(lens[slots[0]]) - 1
+    new = c.table[empty, pos // 16].item()
+    assert new != table[slots[0], pos // 16] and c.refused() == 0
+    layer1 = big[1][far:].view(c.v.shape[1:])
+    for page in (table[slots[0], pos // 16], new):
+        assert torch.equal(layer1[page, pos % 16].flatten(), xs[2][0].bfloat16())
+
+
 def test_attention_refusals(layer):
     rng = np.random.default_rng(2)
     c, slots, bounds, lens, table = build_batch(layer, rng, [[5, 9]], [1], 1, 4, 2, 64, 16, BF16)
