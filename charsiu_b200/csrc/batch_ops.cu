@@ -157,10 +157,11 @@ int append(charsiu_gpu *g, const charsiu_gpu_pages *p, unsigned layer, const int
 	   unsigned n, unsigned t, unsigned n_head, const float *q, const float *k, const float *v,
 	   const float *rope_cs, unsigned n_ctx, void *q_out, void *stream)
 {
-	const uint64_t words = (uint64_t)n * t * (n_head + 2 * p->n_head_kv) * (p->head_dim / 8);
-	return launch(g, stream, pages_append_kernel<T>, dim3((unsigned)((words + 255) / 256)), 256, 0,
-		      *p, (uint32_t)layer, slots, words, (uint32_t)t, (uint32_t)n_head, q, k, v, rope_cs,
-		      (uint32_t)n_ctx, (T *)q_out)
+	// two words a thread, as far as a CTA goes
+	const uint64_t words = (n_head + 2ull * p->n_head_kv) * (p->head_dim / 8), half = (words / 2 + 31) / 32 * 32;
+	const unsigned threads = half < APPEND_MAX_THREADS ? (unsigned)half : APPEND_MAX_THREADS;
+	return launch(g, stream, pages_append_kernel<T>, dim3(n * t), threads, 0, *p, (uint32_t)layer, slots,
+		      (uint32_t)t, (uint32_t)n_head, q, k, v, rope_cs, (uint32_t)n_ctx, (T *)q_out)
 		       ? 0
 		       : -1;
 }
@@ -534,8 +535,7 @@ int charsiu_gpu_pages_append_dev(struct charsiu_gpu *g, const struct charsiu_gpu
 	if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(rope_cs, 16) ||
 	    misaligned(q_out, 16) || misaligned(slots, 4))
 		return refuse(g, "append: an array is misaligned");
-	if ((uint64_t)n * t > 0x7fffffffull || t > 0x7fffffffu ||
-	    (uint64_t)n * t * (n_head + 2ull * p->n_head_kv) * (p->head_dim / 8) > (0x7fffffffull << 8))
+	if ((uint64_t)n * t > 0x7fffffffull || n_head > 1u << 20)
 		return refuse(g, "append: more rows than a call takes");
 	OnDevice on(g);
 	return p->type == TYPE_F16
