@@ -122,6 +122,8 @@ pages_grow_kernel(const __grid_constant__ charsiu_gpu_pages p, const int32_t *__
 			ok = true;
 			have = (uint32_t)((len + p.page - 1) / p.page);
 			need = (uint32_t)((grown + p.page - 1) / p.page) - have;
+			// (more than the pool has is more, however many: the sum of 1024 needs stays in 32 bits)
+			need = need <= p.n_pages ? need : p.n_pages + 1;
 		}
 	}
 	uint32_t total;

@@ -245,6 +245,20 @@ def test_pages_growth_past_every_pool(layer):
     c.same(twin)
 
 
+def test_pages_growths_whose_needs_pass_32_bits(layer):
+    """64 slots that ask for 2^26 pages each, of a pool of 5: the needs add up to 2^32, and all are
+    refused. (The table is as large as told; nothing of it is touched.)"""
+    c = Cache(layer, np.random.default_rng(0), n_seq=64, max_pages=4, n_pages=5, kv=1, layers=1)
+    wide = 1 << 26
+    table = torch.empty(64 * wide, dtype=torch.int32, device="cuda")
+    c.p.table, c.p.max_pages = table.data_ptr(), wide
+    c.grow(range(64), wide * 16)
+    assert c.refused() == 64 and not c.len.any() and not c.ref.any()
+    c.grow([3, 1], 30)
+    assert c.refused() == 64 and c.len.tolist()[:4] == [0, 30, 0, 30] and c.ref.tolist() == [1, 1, 1, 1, 0]
+    assert table[3 * wide:3 * wide + 2].tolist() == [0, 1] and table[wide:wide + 2].tolist() == [2, 3]
+
+
 def test_pages_calls_that_do_nothing(layer):
     c = Cache(layer, np.random.default_rng(1), n_seq=3, max_pages=4, n_pages=5)
     twin = c.plain()
