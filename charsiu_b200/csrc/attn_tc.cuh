@@ -370,7 +370,9 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 	} else {
 		// ---- rows: Q into shared memory first (swizzled as the tensor copies would)
 		const uint32_t rows = halves ? 256 : 128;
-		const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;     // scale > 0 from here on
+		// scale > 0 from here on: Q's sign takes the scale's, and of a scale of 0 Q is 0 (0 times
+		// the -inf of a key behind the end would be NaN)
+		const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale != 0.0f ? 0xffffffffu : 0u;
 		constexpr uint32_t QW = HD / 8, EACH = 128 * QW / 256;      // words a row; a thread's in 128 rows
 		const uint32_t w = threadIdx.x % QW;
 		for (uint32_t r0 = 0; r0 < rows; r0 += 128) {
@@ -385,14 +387,15 @@ attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUten
 			for (uint32_t e = 0; e < EACH; e++) {
 				const uint32_t r = r0 + e * (256 / QW) + threadIdx.x / QW;
 				*(uint4 *)(q_ptr + (w / 8) * q_slab + r * 128 + (((w % 8) ^ (r & 7)) << 4)) =
-					make_uint4(v[e].x ^ flip, v[e].y ^ flip, v[e].z ^ flip, v[e].w ^ flip);
+					make_uint4((v[e].x ^ flip) & keep, (v[e].y ^ flip) & keep, (v[e].z ^ flip) & keep,
+						   (v[e].w ^ flip) & keep);
 			}
 		}
 
 		const uint32_t i = warp / 4, quarter = warp % 4, mine = count(i);
 		const uint32_t lanes = (quarter * 32) << 16, my = s_row[(halves ? i * 128 : 0) + quarter * 32 + lane];
 		const uint32_t ts = tmem + lanes + COL_S + i * 128, to = tmem + lanes + COL_O + i * HD;
-		const float scale = fabsf(a.scale);
+		const float scale = keep ? fabsf(a.scale) : 1.0f;
 		float m = -INFINITY, l = 0.0f;
 		bool ok = true;
 		fence_proxy_async_smem();

@@ -574,6 +574,17 @@ def test_attention_of_many_groups_and_sequences(layer):
         check_attention(c, known, lens, table, t, heads, q, out, scale=scale)
 
 
+def test_attention_with_a_scale_of_0(layer):
+    """The mean of V over the keys that are seen, whichever kernel reads them: a prefix that ends inside a
+    step of the tensor cores', and own keys; the smallest scale too."""
+    rng = np.random.default_rng(34)
+    for scale in (0.0, -0.0, 1e-45):
+        c, slots, bounds, lens, table = build_batch(layer, rng, [[7] * 12], [5], 1, 8, 2, 64, 16, BF16)
+        q = queries(rng, 12, 8, 64, BF16)
+        out = run_attention(layer, c, slots, bounds, [5], 1, 8, q, scale=scale)
+        check_attention(c, slots, lens, table, 1, 8, q, out, scale=scale)
+
+
 def test_attention_of_a_whole_prompt(layer):
     """As many queries as positions, causal: the rows of a prompt, and of one that goes on from shared pages."""
     rng = np.random.default_rng(32)
