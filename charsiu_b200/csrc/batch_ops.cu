@@ -634,6 +634,9 @@ int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_ada
 		s.base = bases ? bases[i] : ys[i];
 		if (!s.y || !s.base || misaligned(s.y, 4) || misaligned(s.base, 4))
 			return refuse(g, "adapters: an output is missing or misaligned");
+		for (unsigned j = 0; j < i; j++)
+			if (s.y == a.s[j].y || s.base == a.s[j].y || s.y == a.s[j].base)
+				return refuse(g, "adapters: two sets share an output, or one's base is another's");
 		s.n = sets[i].n;
 		s.slots = sets[i].slots;
 		s.max_rank = sets[i].max_rank;

@@ -477,7 +477,8 @@ CHARSIU_GPU_API size_t charsiu_gpu_adapters_work(struct charsiu_gpu *g,
  * m rows of the q8_0 activation x = q d that the projections read (q int8 [m][K],
  * d fp32 [m][K/32]), against n <= 8 sets of the same K. bases and ys: n device
  * pointers to fp32 [m][N]; bases[i] may be ys[i], and bases NULL means ys: the
- * projections' outputs get the adapters added. A row whose `which` is no adapter
+ * projections' outputs get the adapters added. No set's output may overlap
+ * another's output or base. A row whose `which` is no adapter
  * (-1) is its base. fp32 products and sums throughout. work: 16-byte aligned, as
  * q is (d 4). */
 CHARSIU_GPU_API int charsiu_gpu_adapters_dev(struct charsiu_gpu *g,

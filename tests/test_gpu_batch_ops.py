@@ -858,6 +858,14 @@ def test_adapters_refusals(layer):
             call(sets(**changes))
     with pytest.raises(GpuError):
         call(sets(count=9))
+    other = torch.zeros(2, 10, device="cuda")
+    two = layer.pointers([y.data_ptr(), other.data_ptr()])
+    call(sets(count=2), ys=two)
+    call(sets(count=2), ys=two, bases=two)
+    with pytest.raises(GpuError):                        # one output of two sets
+        call(sets(count=2), ys=layer.pointers([y.data_ptr()] * 2))
+    with pytest.raises(GpuError):                        # a base that is the other's output
+        call(sets(count=2), ys=two, bases=layer.pointers([other.data_ptr(), y.data_ptr()]))
     for changes in (dict(q=0), dict(q=q.data_ptr() + 8), dict(d=0), dict(which=0), dict(work=0), dict(work_bytes=64),
                     dict(ys=layer.pointers([0])), dict(work=w.data_ptr() + 4), dict(m=(1 << 24) + 1)):
         with pytest.raises(GpuError):
