@@ -97,12 +97,22 @@ __device__ __forceinline__ void adapt_tile(const AdaptArgs &a, const AdaptSet &s
 	}
 }
 
-// two int8 of a word as a pair of T
+// Two int8 of a word, bytes `at` and at + 1, as a pair of T. By their bits: a conversion
+// instruction takes 8 cycles a warp. u = the byte with its sign flipped (value + 128) in the low
+// bits of 1024 (fp16) or 2^23 (fp32) is that plus u, the difference is exact, and so is an
+// int8's bf16, the high half of its fp32.
 template <typename T>
 __device__ __forceinline__ uint32_t int8_pair(uint32_t w, int at)
 {
-	const float lo = (float)(int8_t)(w >> (8 * at)), hi = (float)(int8_t)(w >> (8 * at + 8));
-	return pack_pair<T>(lo, hi);
+	const uint32_t u = w ^ 0x80808080u;
+	if (std::is_same<T, __half>::value) {
+		const uint32_t x = __byte_perm(u, 0x64006400u, at ? 0x5352 : 0x5150);
+		const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&x), __floats2half2_rn(1152.0f, 1152.0f));
+		return *reinterpret_cast<const uint32_t *>(&v);
+	}
+	const float lo = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + at)), 8388736.0f);
+	const float hi = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + at)), 8388736.0f);
+	return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
 }
 
 // t of one tile of rows and one piece of K, for one set. RT: ranks, padded to a
@@ -414,19 +424,19 @@ __device__ __forceinline__ uint32_t adapt_distinct(const int32_t *which, int32_t
 
 template <int RT>
 struct AdaptLong {
-	static constexpr uint32_t A_PITCH = 192;                 // 64 k of a rank; (64 bytes on: other banks)
-	static constexpr uint32_t A_STAGE = RT * A_PITCH;
+	static constexpr uint32_t A_STAGES = 4, A_STAGE = RT * 128;      // 64 k of a rank
 	static constexpr uint32_t B_COLS = 64, B_PITCH = RT * 2 + 16;
 	static constexpr uint32_t B_STAGE = B_COLS * B_PITCH;
 };
 
 template <typename T, int RT>
-__global__ void __launch_bounds__(ADAPT_WARPS * 32)
+__global__ void __launch_bounds__(ADAPT_WARPS * 32, 3)
 adapt_shrink_long_kernel(const __grid_constant__ AdaptArgs a)
 {
 	using L = AdaptLong<RT>;
 	constexpr int NT = RT / 8;
-	__shared__ __align__(16) uint8_t s_a[ADAPT_STAGES][L::A_STAGE];
+	constexpr uint32_t NS = L::A_STAGES;
+	__shared__ __align__(16) uint8_t s_a[NS][L::A_STAGE];
 	__shared__ int32_t s_which[ADAPT_LONG_ROWS], s_list[ADAPT_LONG_ROWS];
 	__shared__ uint32_t s_n;
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
@@ -458,15 +468,16 @@ adapt_shrink_long_kernel(const __grid_constant__ AdaptArgs a)
 	float *t = a.t + (((size_t)blockIdx.z * a.pieces + piece) * a.m + row0) * RT;
 	for (uint32_t j = 0; j < s_n; j++) {
 		const int32_t ad = s_list[j];
-		const uint32_t rank = adapt_rank(set, ad);
+		const uint32_t rank = adapt_rank(set, ad);       // (used at the end only)
 		const uint32_t rows = __ballot_sync(0xffffffffu, mine == ad) & 0xffffu;
 		const T *w = (const T *)set.a + (size_t)ad * set.max_rank * a.k;
 		auto fetch = [&](uint32_t s) {
-			// 8 words of 16 bytes a rank
+			// 8 words of 16 bytes a rank, an odd rank's halves swapped (other banks)
 			for (uint32_t x = threadIdx.x; s < steps && x < RT * 8; x += ADAPT_WARPS * 32) {
 				const uint32_t r = x / 8, k = (s0 + s) * 64 + x % 8 * 8;
-				cp_async16_zero(&s_a[s % ADAPT_STAGES][r * L::A_PITCH + x % 8 * 16],
-						w + (size_t)(r < rank ? r : 0) * a.k + (k < a.k ? k : 0), r < rank && k < a.k);
+				const bool ok = r < set.max_rank && k < a.k;
+				cp_async16_zero(&s_a[s % NS][r * 128 + ((x % 8) ^ (r & 1) * 4) * 16],
+						w + (ok ? (size_t)r * a.k + k : 0), ok);
 			}
 			asm volatile("cp.async.commit_group;" ::: "memory");
 		};
@@ -484,56 +495,68 @@ adapt_shrink_long_kernel(const __grid_constant__ AdaptArgs a)
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
 					const uint32_t block = (s0 + s) * 2 + b;
-					v.x[b][h] = block < nb ? *(const uint2 *)(xq[h] + block * 32) : make_uint2(0, 0);
-					v.d[b][h] = block < nb ? xd[h][block] : 0.0f;
+					const bool ok = s < steps && block < nb;
+					v.x[b][h] = ok ? *(const uint2 *)(xq[h] + block * 32) : make_uint2(0, 0);
+					v.d[b][h] = ok ? xd[h][block] : 0.0f;
 				}
 		};
 		__syncthreads();                  // (the last adapter's stages have been read)
-		Rows now, next;
-		for (uint32_t s = 0; s < ADAPT_STAGES - 1; s++)
+		Rows buf[NS];
+#pragma unroll
+		for (uint32_t s = 0; s < NS - 1; s++) {
 			fetch(s);
-		if (rows && steps)
-			load(now, 0);
-		for (uint32_t s = 0; s < steps; s++) {
-			asm volatile("cp.async.wait_group %0;" :: "n"((int)ADAPT_STAGES - 2) : "memory");
-			__syncthreads();
-			fetch(s + ADAPT_STAGES - 1);
-			if (!rows)
-				continue;
-			if (s + 1 < steps)
-				load(next, s + 1);
-			const uint8_t *stage = s_a[s % ADAPT_STAGES];
+			if (rows)
+				load(buf[s], s);
+		}
+		for (uint32_t s4 = 0; s4 < steps; s4 += NS)
 #pragma unroll
-			for (int b = 0; b < 2; b++) {
-				uint32_t fa[2][4];
+			for (uint32_t u = 0; u < NS; u++) {
+				const uint32_t s = s4 + u;
+				if (s >= steps)
+					break;
+				asm volatile("cp.async.wait_group %0;" :: "n"((int)NS - 2) : "memory");
+				__syncthreads();
+				fetch(s + NS - 1);
+				if (!rows)
+					continue;
+				load(buf[(u + NS - 1) % NS], s + NS - 1);
+				const Rows &now = buf[u];
+				const uint8_t *stage = s_a[u];
 #pragma unroll
-				for (int x = 0; x < 2; x++) {
-					const uint32_t x0 = x ? now.x[b][0].y : now.x[b][0].x, x1 = x ? now.x[b][1].y : now.x[b][1].x;
-					fa[x][0] = int8_pair<T>(x0, 0);
-					fa[x][1] = int8_pair<T>(x1, 0);
-					fa[x][2] = int8_pair<T>(x0, 2);
-					fa[x][3] = int8_pair<T>(x1, 2);
-				}
+				for (int b = 0; b < 2; b++) {
+					uint32_t fa[2][4];
 #pragma unroll
-				for (int n = 0; n < NT; n++) {
-					const uint4 v = *(const uint4 *)(stage + (n * 8 + lane / 4) * L::A_PITCH + b * 64 + c * 16);
-					float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-					mma_16816<T>(sum, fa[0], v.x, v.y);
-					mma_16816<T>(sum, fa[1], v.z, v.w);
+					for (int x = 0; x < 2; x++) {
+						const uint32_t x0 = x ? now.x[b][0].y : now.x[b][0].x, x1 = x ? now.x[b][1].y : now.x[b][1].x;
+						fa[x][0] = int8_pair<T>(x0, 0);
+						fa[x][1] = int8_pair<T>(x1, 0);
+						fa[x][2] = int8_pair<T>(x0, 2);
+						fa[x][3] = int8_pair<T>(x1, 2);
+					}
 #pragma unroll
-					for (int e = 0; e < 4; e++)
-						acc[n][e] = __fmaf_rn(now.d[b][e >> 1], sum[e], acc[n][e]);
+					for (int n = 0; n < NT; n++) {
+						const uint32_t r = n * 8 + lane / 4;
+						const uint4 v = *(const uint4 *)(stage + r * 128 + ((b * 4 + c) ^ (r & 1) * 4) * 16);
+						float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+						mma_16816<T>(sum, fa[0], v.x, v.y);
+						mma_16816<T>(sum, fa[1], v.z, v.w);
+#pragma unroll
+						for (int e = 0; e < 4; e++)
+							acc[n][e] = __fmaf_rn(now.d[b][e >> 1], sum[e], acc[n][e]);
+					}
 				}
 			}
-			now = next;
-		}
 		asm volatile("cp.async.wait_group 0;" ::: "memory");
+		// (what lies behind the rank reached its own columns of t only: 0)
 #pragma unroll
 		for (int n = 0; n < NT; n++)
 #pragma unroll
 			for (int e = 0; e < 4; e += 2)
-				if (rows >> (lane / 4 + 4 * e) & 1)
-					*(float2 *)(t + (lane / 4 + 4 * e) * RT + n * 8 + c * 2) = make_float2(acc[n][e], acc[n][e + 1]);
+				if (rows >> (lane / 4 + 4 * e) & 1) {
+					const uint32_t r = n * 8 + c * 2;
+					*(float2 *)(t + (lane / 4 + 4 * e) * RT + r) =
+						make_float2(r < rank ? acc[n][e] : 0.0f, r + 1 < rank ? acc[n][e + 1] : 0.0f);
+				}
 	}
 }
 
@@ -556,12 +579,33 @@ adapt_sum_kernel(float4 *t, uint32_t pieces, uint32_t each)
 	at[0] = v;
 }
 
+// t as a sum of numbers of B's type, for exact products with B: fp16 in two parts, the row scaled by a
+// power of two so that its largest is in [2^13, 2^14) (what is lost is 2^-24 of a term, or 2^-38
+// of the row's largest), bf16 in three (2^-27). Against two tf32 parts that is 2 or 3 MMAs for 16
+// ranks, not 4 of half the rate, and B needs no conversion.
+template <typename T>
+__host__ __device__ constexpr int adapt_parts()
+{
+	return std::is_same<T, __half>::value ? 2 : 3;
+}
+
+// the power of two for a row whose largest is `top`; 1 where that is 0, inf or NaN
+__device__ __forceinline__ float adapt_lift(float top)
+{
+	const int e = (int)(__float_as_uint(top) >> 23 & 255) - 127;
+	if (!(top > 0.0f) || e == 128)
+		return 1.0f;
+	const int x = min(max(13 - e, -126), 126);
+	return __uint_as_float((uint32_t)(x + 127) << 23);
+}
+
 template <typename T, int RT>
-__global__ void __launch_bounds__(ADAPT_WARPS * 32)
+__global__ void __launch_bounds__(ADAPT_WARPS * 32, 3)
 adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 {
 	using L = AdaptLong<RT>;
-	constexpr int SP = RT / 4, KS = RT / 8;          // ranks a lane; k steps
+	constexpr int SP = RT / 4, PAIRS = SP / 2, KS = RT < 16 ? 1 : RT / 16;      // ranks a lane; k steps
+	constexpr int PARTS = adapt_parts<T>();
 	__shared__ __align__(16) uint8_t s_b[ADAPT_STAGES][L::B_STAGE];
 	__shared__ int32_t s_which[ADAPT_LONG_ROWS], s_list[ADAPT_LONG_ROWS];
 	__shared__ uint32_t s_n;
@@ -584,8 +628,10 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 		if (lane == 0)
 			s_n = n;
 	}
-	// this warp's t, straight into the fragments
-	uint32_t hi[KS][4], lo[KS][4];
+	// this warp's t, straight into the fragments: of the 16 ranks of k step s lane c has ranks
+	// c SP + 4 s ... + 3, of t and of B alike
+	uint32_t part[PARTS][KS][4];
+	float back[2];
 #pragma unroll
 	for (int h = 0; h < 2; h++) {
 		const uint32_t r = row0 + lane / 4 + 8 * h;
@@ -603,11 +649,34 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 					*(float4 *)(v + i) = *(const float4 *)(t + i);
 			}
 		}
+		back[h] = 1.0f;
+		if (PARTS == 2) {
+			float top = 0.0f;
 #pragma unroll
-		for (int i = 0; i < SP; i++) {
-			hi[i / 2][h + 2 * (i % 2)] = __float_as_uint(v[i]) & 0xffffe000u;
-			lo[i / 2][h + 2 * (i % 2)] = __float_as_uint(__fsub_rn(v[i], __uint_as_float(hi[i / 2][h + 2 * (i % 2)])));
+			for (int i = 0; i < SP; i++)
+				top = fmaxf(top, fabsf(v[i]));
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+			const float lift = adapt_lift(top);
+			back[h] = __uint_as_float((254u << 23) - __float_as_uint(lift));      // 1 / lift
+#pragma unroll
+			for (int i = 0; i < SP; i++)
+				v[i] = __fmul_rn(v[i], lift);
 		}
+#pragma unroll
+		for (int p = 0; p < PARTS; p++)
+#pragma unroll
+			for (int i = 0; i < 2 * KS; i++) {
+				uint32_t two = 0;
+				if (i < PAIRS) {
+					two = pack_pair<T>(v[2 * i], v[2 * i + 1]);
+					T x[2];
+					*(uint32_t *)x = two;
+					v[2 * i] = __fsub_rn(v[2 * i], to_float<T>(x[0]));
+					v[2 * i + 1] = __fsub_rn(v[2 * i + 1], to_float<T>(x[1]));
+				}
+				part[p][i / 2][h + 2 * (i % 2)] = two;
+			}
 	}
 	__syncthreads();
 	const int32_t mine = s_which[warp * ADAPT_ROWS + (lane & 15)];
@@ -622,6 +691,10 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 		const float scale = set.scale[ad];
 		const uint32_t rows = __ballot_sync(0xffffffffu, mine == ad) & 0xffffu;
 		const T *w = (const T *)set.b + (size_t)ad * set.n * set.max_rank;
+		uint32_t mask[PAIRS];                     // what is behind the rank counts as 0
+#pragma unroll
+		for (int i = 0; i < PAIRS; i++)
+			mask[i] = (c * SP + 2 * i < rank ? 0xffffu : 0u) | (c * SP + 2 * i + 1 < rank ? 0xffff0000u : 0u);
 		auto fetch = [&](uint32_t s) {
 			for (uint32_t x = threadIdx.x; s < steps && x < L::B_COLS * words; x += ADAPT_WARPS * 32) {
 				const uint32_t r = x / words, i = x - r * words, n = col0 + s * L::B_COLS + r;
@@ -630,22 +703,20 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 			}
 			asm volatile("cp.async.commit_group;" ::: "memory");
 		};
-		__syncthreads();                  // (the last adapter's stages have been read)
-		for (uint32_t s = 0; s < ADAPT_STAGES - 1; s++)
-			fetch(s);
-		for (uint32_t s = 0; s < steps; s++) {
-			// Columns are dealt to the MMAs so that a thread has runs of four: column
-			// 16 x + 4 (n / 2) + 2 (g % 2) + n % 2 is the n-th of group g, x = g / 2, so of
-			// groups 2 x and 2 x + 1 thread c has 16 x + 4 c ... + 3. A row's 64 bytes then
-			// move together (not 32, as in the order of the fragments). The bases of this step are on
-			// their way before its weights are waited for.
-			float base[4][2][4];
-			const uint32_t n0 = col0 + s * L::B_COLS + c * 4;
+		// Columns are dealt to the MMAs so that a thread has runs of four: column
+		// 16 x + 4 (n / 2) + 2 (g % 2) + n % 2 is the n-th of group g, x = g / 2, so of
+		// groups 2 x and 2 x + 1 thread c has 16 x + 4 c ... + 3. A row's 64 bytes then
+		// move together (not 32, as in the order of the fragments). The bases of a step are on
+		// their way from the step before.
+		struct Bases {
+			float v[4][2][4];
+		};
+		auto load = [&](Bases &to, uint32_t s) {
 #pragma unroll
 			for (int x = 0; x < 4; x++)
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
-					const uint32_t r = lane / 4 + 8 * h, col = n0 + x * 16;
+					const uint32_t r = lane / 4 + 8 * h, col = col0 + s * L::B_COLS + c * 4 + x * 16;
 					const float *b = set.base + (size_t)(row0 + r) * set.n + col;
 					const bool mine_too = rows >> r & 1;
 					float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -658,31 +729,41 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 						v.z = col + 2 < end ? b[2] : 0.0f;
 						v.w = col + 3 < end ? b[3] : 0.0f;
 					}
-					*(float4 *)base[x][h] = v;
+					*(float4 *)to.v[x][h] = v;
 				}
+		};
+		__syncthreads();                  // (the last adapter's stages have been read)
+		for (uint32_t s = 0; s < ADAPT_STAGES - 1; s++)
+			fetch(s);
+		auto step = [&](const Bases &now, Bases &next, uint32_t s) {
+			if (s + 1 < steps)
+				load(next, s + 1);
 			asm volatile("cp.async.wait_group %0;" :: "n"((int)ADAPT_STAGES - 2) : "memory");
 			__syncthreads();
 			fetch(s + ADAPT_STAGES - 1);
 			if (!rows)
-				continue;
+				return;
 			const uint8_t *stage = s_b[s % ADAPT_STAGES];
 #pragma unroll
 			for (int x = 0; x < 4; x++) {
 				float acc[2][4], low[2][4];
-				T wv[2][SP];
+				uint32_t wv[2][PAIRS];
 #pragma unroll
 				for (int g = 0; g < 2; g++) {
 					const uint32_t n = lane / 4, col = 16 * x + 4 * (n / 2) + 2 * g + n % 2;
 					const uint8_t *src = stage + col * L::B_PITCH + c * SP * 2;
 #pragma unroll
-					for (int i = 0; i < SP; i += SP < 8 ? SP : 8) {
-						if (SP == 2)
-							*(uint32_t *)wv[g] = *(const uint32_t *)src;
-						else if (SP == 4)
+					for (int i = 0; i < PAIRS; i += PAIRS < 4 ? PAIRS : 4) {
+						if (PAIRS == 1)
+							wv[g][0] = *(const uint32_t *)src;
+						else if (PAIRS == 2)
 							*(uint2 *)wv[g] = *(const uint2 *)src;
 						else
-							*(uint4 *)(wv[g] + i) = *(const uint4 *)(src + i * 2);
+							*(uint4 *)(wv[g] + i) = *(const uint4 *)(src + i * 4);
 					}
+#pragma unroll
+					for (int i = 0; i < PAIRS; i++)
+						wv[g][i] &= mask[i];
 #pragma unroll
 					for (int e = 0; e < 4; e++)
 						acc[g][e] = low[g][e] = 0.0f;
@@ -690,23 +771,22 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 #pragma unroll
 				for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-					for (int g = 0; g < 2; g++) {
-						const uint32_t w0 = c * SP + 2 * ks < rank ? __float_as_uint(to_float<T>(wv[g][2 * ks])) : 0u;
-						const uint32_t w1 =
-							c * SP + 2 * ks + 1 < rank ? __float_as_uint(to_float<T>(wv[g][2 * ks + 1])) : 0u;
-						mma_tf32(low[g], lo[ks], w0, w1);
-						mma_tf32(acc[g], hi[ks], w0, w1);
-					}
+					for (int p = PARTS - 1; p >= 0; p--)
+#pragma unroll
+						for (int g = 0; g < 2; g++)
+							mma_16816<T>(p ? low[g] : acc[g], part[p][ks], wv[g][2 * ks],
+								     2 * ks + 1 < PAIRS ? wv[g][(2 * ks + 1) % PAIRS] : 0u);
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
-					const uint32_t r = lane / 4 + 8 * h, col = n0 + x * 16;
+					const uint32_t r = lane / 4 + 8 * h, col = col0 + s * L::B_COLS + c * 4 + x * 16;
 					if (!(rows >> r & 1))
 						continue;
 					float v[4];
 #pragma unroll
-					for (int e = 0; e < 4; e++)
-						v[e] = __fadd_rn(base[x][h][e],
-								 __fmul_rn(scale, acc[e / 2][2 * h + e % 2] + low[e / 2][2 * h + e % 2]));
+					for (int e = 0; e < 4; e++) {
+						const float sum = acc[e / 2][2 * h + e % 2] + low[e / 2][2 * h + e % 2];
+						v[e] = __fadd_rn(now.v[x][h][e], __fmul_rn(scale, __fmul_rn(sum, back[h])));
+					}
 					float *y = set.y + (size_t)(row0 + r) * set.n + col;
 					if (fours) {
 						if (col < end)
@@ -719,6 +799,14 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 					}
 				}
 			}
+		};
+		// (two buffers by name: a copy of one into the other would wait for its loads)
+		Bases even, odd;
+		load(even, 0);
+		for (uint32_t s = 0; s < steps; s += 2) {
+			step(even, odd, s);
+			if (s + 1 < steps)
+				step(odd, even, s + 1);
 		}
 		asm volatile("cp.async.wait_group 0;" ::: "memory");
 	}
