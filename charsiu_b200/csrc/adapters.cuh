@@ -2,22 +2,24 @@
 // Low-rank adapters of many requests beside a shared projection
 // (charsiu_gpu_adapters_dev): y_r = base_r + scale_a B_a (A_a x_r), a = which[r].
 //
-// Two launches. The first makes t_r = A_a x_r (rank numbers a row): K is cut into
-// pieces whose sums go to scratch. The second adds the pieces up and makes y. Both
-// take tiles of 16 rows, as mma.sync's m. A tile's rows may want different adapters:
-// each of its distinct ones is a product of its own over all 16 rows, of which only
-// the rows that want it are kept (so whatever an adapter's weights are, they reach no
-// other row). In a long prompt a tile has one; in a decode step of many requests they
-// are spread over warps and CTAs.
+// The first launch makes t_r = A_a x_r (rank numbers a row): K is cut into pieces whose sums
+// go to scratch. The last adds the pieces up and makes y (in long batches a launch between
+// them adds up). Both take tiles of 16 rows, as mma.sync's m, in long batches four of them. A
+// tile's rows may want different adapters: each of its distinct ones is a product of its
+// own over all 16 rows, of which only the rows that want it are kept (so whatever an
+// adapter's weights are, they reach no other row). In a long prompt a tile has one; in a
+// decode step of many requests they are spread over warps and CTAs.
 //
-// Bound by memory: an adapter's weights are used for few rows, and y is read and
-// written for rank / 4 multiply-adds a byte.
+// The bytes are few for the time they take (y is read and written for rank / 4 multiply-adds
+// a byte, a decode step's adapters are a few MB): what bounds both is latency. 16 rows, K =
+// N = 2048 and two of 512, rank 16: 12 us, of which two launches of 3 and in each a chain of
+// four dependent loads (which adapter, its rank, its weights, ...). 2000 rows, K = N = 4096,
+// rank 64: 44 us, t 16, its pieces 3, y 25 (66 MB of bases and outputs: 10 us at the copy rate).
 //
-// Precision: x is q d with q int8, exact in both 16-bit types, so a 32-block's
-// products with A are exact and its sum is taken in fp32 before d scales it. t
-// stays fp32: for its product with B it is cut into two tf32 parts of 11 bits each
-// (the second the remainder), and B is exact in tf32, so what is lost is 2^-22 of a
-// term.
+// Precision: x is q d with q int8, exact in both 16-bit types, so a 32-block's products
+// with A are exact and its sum is taken in fp32 before d scales it. t stays fp32: for its
+// product with B it is cut into parts of which each product with B is exact, two of tf32
+// (what is lost is 2^-22 of a term), in long batches two or three of B's type (see there).
 #pragma once
 
 #include "attn.cuh"
@@ -391,8 +393,10 @@ adapt_expand_kernel(const __grid_constant__ AdaptArgs a)
 // The same two steps where there are rows enough: each of four warps has 16 rows, and the
 // adapter's weights pass through shared memory once for all of them (a prompt's rows
 // share their adapter; where they do not, a warp without rows of an adapter sits
-// it out). 2000 rows, K = N = 4096, rank 64: 28 + 58 us by the kernels above, which
-// read every weight again for each 16 rows.
+// it out). 2000 rows, K = N = 4096, rank 64: 16 + 3 + 25 us, against 28 + 58 by the kernels
+// above, which read every weight again for each 16 rows. Adapters one at a time, not two:
+// 48 us for that, 145 against 113 for 1000 rows of 8 mixed adapters (but 38 against 42 for
+// 2000 rows of one).
 constexpr uint32_t ADAPT_LONG_ROWS = 64, ADAPT_STAGES = 3;
 
 __device__ __forceinline__ void cp_async16_zero(void *dst, const void *src, bool ok)
@@ -422,12 +426,46 @@ __device__ __forceinline__ uint32_t adapt_distinct(const int32_t *which, int32_t
 	return __popc(firsts0) + __popc(firsts1);
 }
 
+// The weights of two of the tile's adapters pass together (a tile where one request's rows end
+// and the next one's begin takes as long as others so): each warp takes those that
+// its rows want.
+constexpr uint32_t ADAPT_PASS = 2;
+
 template <int RT>
 struct AdaptLong {
-	static constexpr uint32_t A_STAGES = 4, A_STAGE = RT * 128;      // 64 k of a rank
+	static constexpr uint32_t A_STAGES = 3, A_PART = RT * 128, A_STAGE = ADAPT_PASS * A_PART;      // 64 k of a rank
 	static constexpr uint32_t B_COLS = 64, B_PITCH = RT * 2 + 16;
-	static constexpr uint32_t B_STAGE = B_COLS * B_PITCH;
+	static constexpr uint32_t B_PART = B_COLS * B_PITCH, B_STAGE = ADAPT_PASS * B_PART;
+	static constexpr size_t A_SMEM = A_STAGES * A_STAGE, B_SMEM = ADAPT_STAGES * B_STAGE;
 };
+
+struct AdaptLongTile {
+	int32_t which[ADAPT_LONG_ROWS], list[ADAPT_LONG_ROWS];
+	uint32_t rank[ADAPT_LONG_ROWS];
+	float scale[ADAPT_LONG_ROWS];
+	uint32_t n;
+};
+
+// by the CTA; ends with a barrier
+__device__ __forceinline__ void adapt_long_tile(const AdaptArgs &a, const AdaptSet &s, uint32_t tile0,
+						AdaptLongTile &t)
+{
+	const uint32_t lane = threadIdx.x & 31;
+	if (threadIdx.x < ADAPT_LONG_ROWS)
+		t.which[threadIdx.x] = adapt_which(a, s, tile0 + threadIdx.x);
+	__syncthreads();
+	if (threadIdx.x < 32) {
+		const uint32_t n = adapt_distinct(t.which, t.list);
+		__syncwarp();
+		for (uint32_t j = lane; j < n; j += 32) {
+			t.rank[j] = adapt_rank(s, t.list[j]);
+			t.scale[j] = s.scale[t.list[j]];
+		}
+		if (lane == 0)
+			t.n = n;
+	}
+	__syncthreads();
+}
 
 template <typename T, int RT>
 __global__ void __launch_bounds__(ADAPT_WARPS * 32, 3)
@@ -436,27 +474,18 @@ adapt_shrink_long_kernel(const __grid_constant__ AdaptArgs a)
 	using L = AdaptLong<RT>;
 	constexpr int NT = RT / 8;
 	constexpr uint32_t NS = L::A_STAGES;
-	__shared__ __align__(16) uint8_t s_a[NS][L::A_STAGE];
-	__shared__ int32_t s_which[ADAPT_LONG_ROWS], s_list[ADAPT_LONG_ROWS];
-	__shared__ uint32_t s_n;
+	extern __shared__ __align__(128) uint8_t adapt_raw[];
+	__shared__ AdaptLongTile s_tile;
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
 	const uint32_t tile0 = blockIdx.x * ADAPT_LONG_ROWS, row0 = tile0 + warp * ADAPT_ROWS, piece = blockIdx.y;
 	const AdaptSet &set = a.s[blockIdx.z];
 	pdl_wait();
 	pdl_launch_dependents();
-	if (threadIdx.x < ADAPT_LONG_ROWS)
-		s_which[threadIdx.x] = adapt_which(a, set, tile0 + threadIdx.x);
-	__syncthreads();
-	if (warp == 0) {
-		const uint32_t n = adapt_distinct(s_which, s_list);
-		if (lane == 0)
-			s_n = n;
-	}
-	__syncthreads();
+	adapt_long_tile(a, set, tile0, s_tile);
 	// the piece in steps of two 32-blocks
 	const uint32_t nb = a.k / 32, steps_all = (nb + 1) / 2, each = (steps_all + a.pieces - 1) / a.pieces;
 	const uint32_t s0 = min(piece * each, steps_all), steps = min(s0 + each, steps_all) - s0;
-	const int32_t mine = s_which[warp * ADAPT_ROWS + (lane & 15)];
+	const int32_t mine = s_tile.which[warp * ADAPT_ROWS + (lane & 15)];
 	const int8_t *xq[2];
 	const float *xd[2];
 #pragma unroll
@@ -466,18 +495,20 @@ adapt_shrink_long_kernel(const __grid_constant__ AdaptArgs a)
 		xd[h] = a.d + (size_t)r * nb;
 	}
 	float *t = a.t + (((size_t)blockIdx.z * a.pieces + piece) * a.m + row0) * RT;
-	for (uint32_t j = 0; j < s_n; j++) {
-		const int32_t ad = s_list[j];
-		const uint32_t rank = adapt_rank(set, ad);       // (used at the end only)
-		const uint32_t rows = __ballot_sync(0xffffffffu, mine == ad) & 0xffffu;
-		const T *w = (const T *)set.a + (size_t)ad * set.max_rank * a.k;
+	for (uint32_t j = 0; j < s_tile.n; j += ADAPT_PASS) {
+		const uint32_t two = min(s_tile.n - j, ADAPT_PASS);
+		const int32_t ad0 = s_tile.list[j], ad1 = two > 1 ? s_tile.list[j + 1] : -2;
+		const uint32_t rows0 = __ballot_sync(0xffffffffu, mine == ad0) & 0xffffu;
+		const uint32_t rows1 = __ballot_sync(0xffffffffu, mine == ad1) & 0xffffu;
+		const uint32_t rows = rows0 | rows1;
 		auto fetch = [&](uint32_t s) {
 			// 8 words of 16 bytes a rank, an odd rank's halves swapped (other banks)
-			for (uint32_t x = threadIdx.x; s < steps && x < RT * 8; x += ADAPT_WARPS * 32) {
-				const uint32_t r = x / 8, k = (s0 + s) * 64 + x % 8 * 8;
+			for (uint32_t x = threadIdx.x; s < steps && x < two * RT * 8; x += ADAPT_WARPS * 32) {
+				const uint32_t r = x / 8 % RT, k = (s0 + s) * 64 + x % 8 * 8;
 				const bool ok = r < set.max_rank && k < a.k;
-				cp_async16_zero(&s_a[s % NS][r * 128 + ((x % 8) ^ (r & 1) * 4) * 16],
-						w + (ok ? (size_t)r * a.k + k : 0), ok);
+				const size_t row = (size_t)(x / 8 < RT ? ad0 : ad1) * set.max_rank + (ok ? r : 0);
+				cp_async16_zero(adapt_raw + s % NS * L::A_STAGE + x / 8 * 128 + ((x % 8) ^ (r & 1) * 4) * 16,
+						(const T *)set.a + row * a.k + (ok ? k : 0), ok);
 			}
 			asm volatile("cp.async.commit_group;" ::: "memory");
 		};
@@ -500,7 +531,7 @@ adapt_shrink_long_kernel(const __grid_constant__ AdaptArgs a)
 					v.d[b][h] = ok ? xd[h][block] : 0.0f;
 				}
 		};
-		__syncthreads();                  // (the last adapter's stages have been read)
+		__syncthreads();                  // (the last adapters' stages have been read)
 		Rows buf[NS];
 #pragma unroll
 		for (uint32_t s = 0; s < NS - 1; s++) {
@@ -521,42 +552,52 @@ adapt_shrink_long_kernel(const __grid_constant__ AdaptArgs a)
 					continue;
 				load(buf[(u + NS - 1) % NS], s + NS - 1);
 				const Rows &now = buf[u];
-				const uint8_t *stage = s_a[u];
+				uint32_t fa[2][2][4];
 #pragma unroll
-				for (int b = 0; b < 2; b++) {
-					uint32_t fa[2][4];
+				for (int b = 0; b < 2; b++)
 #pragma unroll
 					for (int x = 0; x < 2; x++) {
 						const uint32_t x0 = x ? now.x[b][0].y : now.x[b][0].x, x1 = x ? now.x[b][1].y : now.x[b][1].x;
-						fa[x][0] = int8_pair<T>(x0, 0);
-						fa[x][1] = int8_pair<T>(x1, 0);
-						fa[x][2] = int8_pair<T>(x0, 2);
-						fa[x][3] = int8_pair<T>(x1, 2);
+						fa[b][x][0] = int8_pair<T>(x0, 0);
+						fa[b][x][1] = int8_pair<T>(x1, 0);
+						fa[b][x][2] = int8_pair<T>(x0, 2);
+						fa[b][x][3] = int8_pair<T>(x1, 2);
 					}
+#pragma unroll 1
+				for (uint32_t g = 0; g < two; g++) {
+					const uint32_t in = g ? rows1 : rows0;
+					if (!in)
+						continue;
+					const bool take[2] = {(in >> (lane / 4) & 1) != 0, (in >> (lane / 4 + 8) & 1) != 0};
+					const uint8_t *stage = adapt_raw + u * L::A_STAGE + g * L::A_PART;
 #pragma unroll
-					for (int n = 0; n < NT; n++) {
-						const uint32_t r = n * 8 + lane / 4;
-						const uint4 v = *(const uint4 *)(stage + r * 128 + ((b * 4 + c) ^ (r & 1) * 4) * 16);
-						float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-						mma_16816<T>(sum, fa[0], v.x, v.y);
-						mma_16816<T>(sum, fa[1], v.z, v.w);
+					for (int b = 0; b < 2; b++)
 #pragma unroll
-						for (int e = 0; e < 4; e++)
-							acc[n][e] = __fmaf_rn(now.d[b][e >> 1], sum[e], acc[n][e]);
-					}
+						for (int n = 0; n < NT; n++) {
+							const uint32_t r = n * 8 + lane / 4;
+							const uint4 v = *(const uint4 *)(stage + r * 128 + ((b * 4 + c) ^ (r & 1) * 4) * 16);
+							float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+							mma_16816<T>(sum, fa[b][0], v.x, v.y);
+							mma_16816<T>(sum, fa[b][1], v.z, v.w);
+#pragma unroll
+							for (int e = 0; e < 4; e++)
+								acc[n][e] = take[e >> 1] ? __fmaf_rn(now.d[b][e >> 1], sum[e], acc[n][e]) : acc[n][e];
+						}
 				}
 			}
 		asm volatile("cp.async.wait_group 0;" ::: "memory");
-		// (what lies behind the rank reached its own columns of t only: 0)
+		// (what lies behind a rank reached its own columns of t only: 0)
 #pragma unroll
-		for (int n = 0; n < NT; n++)
+		for (int h = 0; h < 2; h++) {
+			const uint32_t r = lane / 4 + 8 * h, rank = s_tile.rank[j + (rows1 >> r & 1)];
+			if (rows >> r & 1)
 #pragma unroll
-			for (int e = 0; e < 4; e += 2)
-				if (rows >> (lane / 4 + 4 * e) & 1) {
-					const uint32_t r = n * 8 + c * 2;
-					*(float2 *)(t + (lane / 4 + 4 * e) * RT + r) =
-						make_float2(r < rank ? acc[n][e] : 0.0f, r + 1 < rank ? acc[n][e + 1] : 0.0f);
+				for (int n = 0; n < NT; n++) {
+					const uint32_t i = n * 8 + c * 2;
+					*(float2 *)(t + r * RT + i) = make_float2(i < rank ? acc[n][2 * h] : 0.0f,
+										  i + 1 < rank ? acc[n][2 * h + 1] : 0.0f);
 				}
+		}
 	}
 }
 
@@ -606,9 +647,8 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 	using L = AdaptLong<RT>;
 	constexpr int SP = RT / 4, PAIRS = SP / 2, KS = RT < 16 ? 1 : RT / 16;      // ranks a lane; k steps
 	constexpr int PARTS = adapt_parts<T>();
-	__shared__ __align__(16) uint8_t s_b[ADAPT_STAGES][L::B_STAGE];
-	__shared__ int32_t s_which[ADAPT_LONG_ROWS], s_list[ADAPT_LONG_ROWS];
-	__shared__ uint32_t s_n;
+	extern __shared__ __align__(128) uint8_t adapt_raw[];
+	__shared__ AdaptLongTile s_tile;
 	const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
 	const uint32_t tile0 = blockIdx.x * ADAPT_LONG_ROWS, row0 = tile0 + warp * ADAPT_ROWS;
 	uint32_t si = 0;
@@ -620,14 +660,7 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 	const bool fours = set.n % 4 == 0 && !(((uintptr_t)set.base | (uintptr_t)set.y) & 15);
 	pdl_wait();
 	pdl_launch_dependents();
-	if (threadIdx.x < ADAPT_LONG_ROWS)
-		s_which[threadIdx.x] = adapt_which(a, set, tile0 + threadIdx.x);
-	__syncthreads();
-	if (warp == 0) {
-		const uint32_t n = adapt_distinct(s_which, s_list);
-		if (lane == 0)
-			s_n = n;
-	}
+	adapt_long_tile(a, set, tile0, s_tile);
 	// this warp's t, straight into the fragments: of the 16 ranks of k step s lane c has ranks
 	// c SP + 4 s ... + 3, of t and of B alike
 	uint32_t part[PARTS][KS][4];
@@ -678,28 +711,28 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 				part[p][i / 2][h + 2 * (i % 2)] = two;
 			}
 	}
-	__syncthreads();
-	const int32_t mine = s_which[warp * ADAPT_ROWS + (lane & 15)];
+	const int32_t mine = s_tile.which[warp * ADAPT_ROWS + (lane & 15)];
 	const uint32_t wants = __ballot_sync(0xffffffffu, mine >= 0) & 0xffffu;
 	// rows of no adapter keep the base's bits
 	const uint32_t there = row0 >= a.m ? 0 : a.m - row0 < ADAPT_ROWS ? (1u << (a.m - row0)) - 1 : 0xffffu;
 	adapt_copy(set, row0, there & ~wants, col0, end, lane, 32);
-	const uint32_t words = set.max_rank / 8;          // of 16 bytes a column
-	for (uint32_t j = 0; j < s_n; j++) {
-		const int32_t ad = s_list[j];
-		const uint32_t rank = adapt_rank(set, ad);
-		const float scale = set.scale[ad];
-		const uint32_t rows = __ballot_sync(0xffffffffu, mine == ad) & 0xffffu;
-		const T *w = (const T *)set.b + (size_t)ad * set.n * set.max_rank;
-		uint32_t mask[PAIRS];                     // what is behind the rank counts as 0
-#pragma unroll
-		for (int i = 0; i < PAIRS; i++)
-			mask[i] = (c * SP + 2 * i < rank ? 0xffffu : 0u) | (c * SP + 2 * i + 1 < rank ? 0xffff0000u : 0u);
+	for (uint32_t j = 0; j < s_tile.n; j += ADAPT_PASS) {
+		const uint32_t two = min(s_tile.n - j, ADAPT_PASS);
+		const int32_t ad0 = s_tile.list[j], ad1 = two > 1 ? s_tile.list[j + 1] : -2;
+		const uint32_t rows0 = __ballot_sync(0xffffffffu, mine == ad0) & 0xffffu;
+		const uint32_t rows1 = __ballot_sync(0xffffffffu, mine == ad1) & 0xffffu;
+		const uint32_t rows = rows0 | rows1;
+		// what is behind a rank counts as 0: words of 8 by the copies, the rest by hand
+		const uint32_t rank0 = s_tile.rank[j], rank1 = two > 1 ? s_tile.rank[j + 1] : 0;
+		const bool ragged = (rank0 | rank1) % 8;
 		auto fetch = [&](uint32_t s) {
-			for (uint32_t x = threadIdx.x; s < steps && x < L::B_COLS * words; x += ADAPT_WARPS * 32) {
-				const uint32_t r = x / words, i = x - r * words, n = col0 + s * L::B_COLS + r;
-				cp_async16_zero(&s_b[s % ADAPT_STAGES][r * L::B_PITCH + i * 16],
-						w + (size_t)(n < end ? n : col0) * set.max_rank + i * 8, n < end);
+			constexpr uint32_t WORDS = RT / 8;
+			for (uint32_t x = threadIdx.x; s < steps && x < two * L::B_COLS * WORDS; x += ADAPT_WARPS * 32) {
+				const uint32_t r = x / WORDS, i = x % WORDS, n = col0 + s * L::B_COLS + r % L::B_COLS;
+				const bool first = r < L::B_COLS, ok = n < end && i * 8 < (first ? rank0 : rank1);
+				const size_t col = (size_t)(first ? ad0 : ad1) * set.n + (ok ? n : 0);
+				cp_async16_zero(adapt_raw + s % ADAPT_STAGES * L::B_STAGE + r * L::B_PITCH + i * 16,
+						(const T *)set.b + col * set.max_rank + (ok ? i * 8 : 0), ok);
 			}
 			asm volatile("cp.async.commit_group;" ::: "memory");
 		};
@@ -732,7 +765,7 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 					*(float4 *)to.v[x][h] = v;
 				}
 		};
-		__syncthreads();                  // (the last adapter's stages have been read)
+		__syncthreads();                  // (the last adapters' stages have been read)
 		for (uint32_t s = 0; s < ADAPT_STAGES - 1; s++)
 			fetch(s);
 		auto step = [&](const Bases &now, Bases &next, uint32_t s) {
@@ -740,62 +773,73 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 				load(next, s + 1);
 			asm volatile("cp.async.wait_group %0;" :: "n"((int)ADAPT_STAGES - 2) : "memory");
 			__syncthreads();
-			fetch(s + ADAPT_STAGES - 1);
-			if (!rows)
-				return;
-			const uint8_t *stage = s_b[s % ADAPT_STAGES];
-#pragma unroll
-			for (int x = 0; x < 4; x++) {
-				float acc[2][4], low[2][4];
-				uint32_t wv[2][PAIRS];
-#pragma unroll
-				for (int g = 0; g < 2; g++) {
-					const uint32_t n = lane / 4, col = 16 * x + 4 * (n / 2) + 2 * g + n % 2;
-					const uint8_t *src = stage + col * L::B_PITCH + c * SP * 2;
-#pragma unroll
-					for (int i = 0; i < PAIRS; i += PAIRS < 4 ? PAIRS : 4) {
-						if (PAIRS == 1)
-							wv[g][0] = *(const uint32_t *)src;
-						else if (PAIRS == 2)
-							*(uint2 *)wv[g] = *(const uint2 *)src;
-						else
-							*(uint4 *)(wv[g] + i) = *(const uint4 *)(src + i * 4);
-					}
-#pragma unroll
-					for (int i = 0; i < PAIRS; i++)
-						wv[g][i] &= mask[i];
-#pragma unroll
-					for (int e = 0; e < 4; e++)
-						acc[g][e] = low[g][e] = 0.0f;
+			uint8_t *stage0 = adapt_raw + s % ADAPT_STAGES * L::B_STAGE;
+			if (ragged) {
+				for (uint32_t r = threadIdx.x; r < two * L::B_COLS; r += ADAPT_WARPS * 32) {
+					const uint32_t rank = r < L::B_COLS ? rank0 : rank1;
+					for (uint32_t i = rank; i % 8; i++)
+						*(uint16_t *)(stage0 + r * L::B_PITCH + i * 2) = 0;
 				}
+				__syncthreads();
+			}
+			fetch(s + ADAPT_STAGES - 1);
+#pragma unroll 1
+			for (uint32_t which = 0; which < two; which++) {
+				const uint32_t in = which ? rows1 : rows0;
+				if (!in)
+					continue;
+				const float scale = s_tile.scale[j + which];
+				const uint8_t *stage = stage0 + which * L::B_PART;
 #pragma unroll
-				for (int ks = 0; ks < KS; ks++)
+				for (int x = 0; x < 4; x++) {
+					float acc[2][4], low[2][4];
+					uint32_t wv[2][PAIRS];
 #pragma unroll
-					for (int p = PARTS - 1; p >= 0; p--)
+					for (int g = 0; g < 2; g++) {
+						const uint32_t n = lane / 4, col = 16 * x + 4 * (n / 2) + 2 * g + n % 2;
+						const uint8_t *src = stage + col * L::B_PITCH + c * SP * 2;
 #pragma unroll
-						for (int g = 0; g < 2; g++)
-							mma_16816<T>(p ? low[g] : acc[g], part[p][ks], wv[g][2 * ks],
-								     2 * ks + 1 < PAIRS ? wv[g][(2 * ks + 1) % PAIRS] : 0u);
-#pragma unroll
-				for (int h = 0; h < 2; h++) {
-					const uint32_t r = lane / 4 + 8 * h, col = col0 + s * L::B_COLS + c * 4 + x * 16;
-					if (!(rows >> r & 1))
-						continue;
-					float v[4];
-#pragma unroll
-					for (int e = 0; e < 4; e++) {
-						const float sum = acc[e / 2][2 * h + e % 2] + low[e / 2][2 * h + e % 2];
-						v[e] = __fadd_rn(now.v[x][h][e], __fmul_rn(scale, __fmul_rn(sum, back[h])));
-					}
-					float *y = set.y + (size_t)(row0 + r) * set.n + col;
-					if (fours) {
-						if (col < end)
-							*(float4 *)y = make_float4(v[0], v[1], v[2], v[3]);
-					} else {
+						for (int i = 0; i < PAIRS; i += PAIRS < 4 ? PAIRS : 4) {
+							if (PAIRS == 1)
+								wv[g][0] = *(const uint32_t *)src;
+							else if (PAIRS == 2)
+								*(uint2 *)wv[g] = *(const uint2 *)src;
+							else
+								*(uint4 *)(wv[g] + i) = *(const uint4 *)(src + i * 4);
+						}
 #pragma unroll
 						for (int e = 0; e < 4; e++)
-							if (col + e < end)
-								y[e] = v[e];
+							acc[g][e] = low[g][e] = 0.0f;
+					}
+#pragma unroll
+					for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+						for (int p = PARTS - 1; p >= 0; p--)
+#pragma unroll
+							for (int g = 0; g < 2; g++)
+								mma_16816<T>(p ? low[g] : acc[g], part[p][ks], wv[g][2 * ks],
+									     2 * ks + 1 < PAIRS ? wv[g][(2 * ks + 1) % PAIRS] : 0u);
+#pragma unroll
+					for (int h = 0; h < 2; h++) {
+						const uint32_t r = lane / 4 + 8 * h, col = col0 + s * L::B_COLS + c * 4 + x * 16;
+						if (!(in >> r & 1))
+							continue;
+						float v[4];
+#pragma unroll
+						for (int e = 0; e < 4; e++) {
+							const float sum = acc[e / 2][2 * h + e % 2] + low[e / 2][2 * h + e % 2];
+							v[e] = __fadd_rn(now.v[x][h][e], __fmul_rn(scale, __fmul_rn(sum, back[h])));
+						}
+						float *y = set.y + (size_t)(row0 + r) * set.n + col;
+						if (fours) {
+							if (col < end)
+								*(float4 *)y = make_float4(v[0], v[1], v[2], v[3]);
+						} else {
+#pragma unroll
+							for (int e = 0; e < 4; e++)
+								if (col + e < end)
+									y[e] = v[e];
+						}
 					}
 				}
 			}

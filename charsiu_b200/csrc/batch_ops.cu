@@ -333,16 +333,17 @@ uint32_t adapters_ranks(const charsiu_gpu_adapters *s, unsigned n)
 constexpr uint32_t ADAPT_CTAS_PER_SM = 4, ADAPT_MAX_PIECES = 16, ADAPT_LONG_CTAS_PER_SM = 3;
 constexpr unsigned ADAPT_LONG_M = 512;
 
-// Whether the rows go 64 to a CTA. Measured, K = N = 4096, 16 rows a CTA against 64: 256 rows of
-// rank 16 13 against 20 us, of rank 64 35 against 34; 512 rows 18 against 18, and 46 against 34;
-// 1000 rows 31 against 27, and 56 against 42. With the rows' adapters mixed, 256 rows 32 against
-// 40 us, 1000 rows 99 against 76.
+// Whether the rows go 64 to a CTA. Measured, K = N = 4096, 16 rows a CTA against 64: of rank 16
+// 256 rows 13 against 19 us, 512 rows 18 against 18, 1000 rows 31 against 29; of rank 64 128 rows
+// 31 against 33, 256 rows 35 against 28, 512 rows 46 against 32, 1000 rows 56 against 38. With the
+// rows' adapters mixed, 256 rows of rank 16 32 against 35 us, of rank 64 68 against 56.
 bool adapters_long(const charsiu_gpu_adapters *s, unsigned n, unsigned m)
 {
 	for (unsigned i = 0; i < n; i++)
 		if (s[i].max_rank % 8)          // (weights are copied by 16 bytes)
 			return false;
-	return m >= ADAPT_LONG_M && adapters_ranks(s, n) <= 64;
+	const uint32_t ranks = adapters_ranks(s, n);
+	return ranks <= 64 && m >= (ranks == 64 ? ADAPT_LONG_M / 2 : ADAPT_LONG_M);
 }
 
 // pieces of K: enough CTAs to fill the GPU, at least one 32-block a warp
@@ -374,13 +375,17 @@ int adapters(charsiu_gpu *g, const AdaptArgs &a, bool lng, void *stream)
 		if (lng) {
 			const unsigned tiles = (a.m + ADAPT_LONG_ROWS - 1) / ADAPT_LONG_ROWS;
 			const uint32_t each = a.m * (RT / 4);
-			return launch(g, stream, adapt_shrink_long_kernel<T, RT>, dim3(tiles, a.pieces, a.n_sets),
-				      ADAPT_WARPS * 32, 0, a) &&
+			constexpr size_t a_smem = AdaptLong<RT>::A_SMEM, b_smem = AdaptLong<RT>::B_SMEM;
+			static std::atomic<uint64_t> a_done, b_done;
+			return allow_smem(g, adapt_shrink_long_kernel<T, RT>, a_smem, a_done) &&
+					       allow_smem(g, adapt_expand_long_kernel<T, RT>, b_smem, b_done) &&
+					       launch(g, stream, adapt_shrink_long_kernel<T, RT>,
+						      dim3(tiles, a.pieces, a.n_sets), ADAPT_WARPS * 32, a_smem, a) &&
 					       (a.pieces == 1 ||
 						launch(g, stream, adapt_sum_kernel, dim3((each + 255) / 256, a.n_sets), 256, 0,
 						       (float4 *)a.t, a.pieces, each)) &&
 					       launch(g, stream, adapt_expand_long_kernel<T, RT>, dim3(tiles, a.blocks),
-						      ADAPT_WARPS * 32, 0, a)
+						      ADAPT_WARPS * 32, b_smem, a)
 				       ? 0
 				       : -1;
 		}
@@ -648,9 +653,10 @@ int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_ada
 	const uint64_t tile = lng ? ADAPT_LONG_ROWS : ADAPT_ROWS, tiles = (m + tile - 1) / tile;
 	const uint64_t aim = (uint64_t)(lng ? ADAPT_LONG_CTAS_PER_SM : ADAPT_CTAS_PER_SM) * layer_sms(g);
 	if (lng) {
-		// (narrower than fills it: a tile of several adapters takes as many times as long)
-		a.cols = (uint32_t)((tiles * columns / (2 * aim) + 63) / 64 * 64);
-		a.cols = a.cols < 64 ? 64 : a.cols > 512 ? 512 : a.cols;
+		// (as many as are on it at once: twice as many, of half the columns, take 2000 rows of
+		// rank 64 from 45 to 48 us, 1000 of mixed adapters from 113 to 128)
+		a.cols = (uint32_t)((tiles * columns / aim + 63) / 64 * 64);
+		a.cols = a.cols < 64 ? 64 : a.cols > 1024 ? 1024 : a.cols;
 	} else {
 		a.cols = 256;
 		while (a.cols > 32 && tiles * columns / a.cols < aim)

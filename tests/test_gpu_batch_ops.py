@@ -793,7 +793,7 @@ def check_adapters(q, d, which, mats, ranks, scale, bases, ys):
     (16, 1024, [129], 16, 24, F16), (17, 512, [64, 1], 3, 64, BF16), (33, 2048, [300], 40, 32, BF16),
     (70, 256, [1000], 2, 128, F16), (40, 128, [33], 5, 104, BF16), (600, 160, [96], 3, 40, F16),
     (5, 14336, [48], 5, 16, BF16), (560, 992, [130, 7], 70, 16, BF16), (513, 64, [64], 1, 8, F16),
-    (530, 320, [201, 66], 4, 64, BF16), (520, 32, [40], 3, 4, F16), (515, 96, [68], 2, 128, BF16)])
+    (530, 320, [201, 66], 4, 64, BF16), (300, 192, [130, 64], 3, 64, F16), (257, 64, [36], 9, 48, F16), (520, 32, [40], 3, 4, F16), (515, 96, [68], 2, 128, BF16)])
 def test_adapters(layer, m, k, ns, slots, max_rank, ty):
     rng = np.random.default_rng(m + k)
     mats, ranks, scale = make_adapters(rng, slots, max_rank, k, ns, ty)
@@ -825,6 +825,43 @@ def test_adapters_rows_keep_apart(layer):
     got = run_adapters(layer, mats, [16, 3, 0, 999, -3], scale, q, d, which, [base])
     rows = [r for r in range(m) if which[r] != 0 and r != 5]
     assert np.array_equal(clean[0][rows], got[0][rows])
+
+
+def test_adapters_rows_keep_apart_in_long_batches(layer):
+    """The same where four tiles of rows pass together, two adapters at a time."""
+    rng = np.random.default_rng(5)
+    m, k, n = 600, 160, 68
+    for ty in (F16, BF16):
+        mats, _, scale = make_adapters(rng, 5, 16, k, [n], ty, ranks=[16, 3, 16, 16, 16])
+        q = rng.integers(-127, 128, (m, k)).astype(np.int8)
+        d = np.full((m, k // 32), 0.01, np.float32)
+        base = rng.standard_normal((m, n)).astype(np.float32)
+        which = [i % 5 - (i > 400) for i in range(m)]
+        clean = run_adapters(layer, mats, [16, 3, 0, 999, -3], scale, q, d, which, [base], ty=ty)
+        check_adapters(q, d, which, mats, [16, 3, 0, 16, 0], scale, [base], clean)
+        mats[0][0][0] = float("nan")
+        mats[0][1][0] = float("inf")
+        d[5] = np.inf
+        got = run_adapters(layer, mats, [16, 3, 0, 999, -3], scale, q, d, which, [base], ty=ty)
+        rows = [r for r in range(m) if which[r] != 0 and r != 5]
+        assert np.array_equal(clean[0][rows], got[0][rows])
+
+
+@pytest.mark.parametrize("ty", [BF16, F16])
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 1e4, 1e18])
+def test_adapters_of_any_size_of_activation(layer, ty, size):
+    """t far below and above what 16 bits hold, within a row too."""
+    rng = np.random.default_rng(6)
+    m, k, n, r = 520, 64, 72, 16
+    mats, ranks, scale = make_adapters(rng, 2, r, k, [n], ty, ranks=[r, r])
+    for s in range(2):
+        mats[0][0][s] *= torch.tensor([10.0 ** (-i / 4) for i in range(r)])[:, None]
+    q = rng.integers(-127, 128, (m, k)).astype(np.int8)
+    d = (size * (0.1 + rng.random((m, k // 32)))).astype(np.float32)
+    base = np.zeros((m, n), np.float32)
+    which = rng.integers(0, 2, m).tolist()
+    check_adapters(q, d, which, mats, ranks, scale, [base],
+                   run_adapters(layer, mats, ranks, scale, q, d, which, [base], ty=ty))
 
 
 def test_adapters_refusals(layer):
