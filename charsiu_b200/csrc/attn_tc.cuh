@@ -28,6 +28,14 @@
 // and descriptors put together in 64 bits for each cost 120 to 170. Here a descriptor's
 // high word is a constant and its low word a running sum.
 //
+// What bounds it: a step of 2 x 128 rows by 64 keys takes 0.9 us, of which 0.54 are the
+// exponentials alone and 0.68 the MMAs alone; they overlap across the two streams but not with
+// a stream's own tensor memory loads. 64 sequences of 4 rows on 16384 keys, 8 KV heads of 128, on 88
+// multiprocessors: 38 us, 17.2 GFLOP, 450 TFLOP/s (0.45 of those multiprocessors' share of
+// the measured bf16 rate), every key read once (67 MB). With scores of 128 keys in one
+// buffer a tile takes 2.4 us, not 1.8; with two threads a row the whole spills, 38 against
+// 31 us at that time.
+//
 // O is scaled only where a row's maximum has grown by more than 2^8 since it was
 // last taken (P stays below 2^8, exact enough in both types); the weight of the
 // piece is taken with the same maximum, so the result is the same.
