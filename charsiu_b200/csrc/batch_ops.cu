@@ -168,6 +168,10 @@ int append(charsiu_gpu *g, const charsiu_gpu_pages *p, unsigned layer, const int
 
 // ---- attention ------------------------------------------------------------------
 
+// Every CTA looks its group up among all, and a group's shared length among its sequences: with
+// these at their most that is 0.1 ms an item (2^25 sequences in as many groups would take hours).
+constexpr uint32_t ATTN_MAX_SEQS = 65536, ATTN_MAX_GROUPS = 4096;
+
 const char *attention_fault(const charsiu_gpu_pages *p, const charsiu_gpu_attention *a)
 {
 	const char *why = pages_fault(p);
@@ -177,7 +181,8 @@ const char *attention_fault(const charsiu_gpu_pages *p, const charsiu_gpu_attent
 		return "the batch lacks an array";
 	if (!a->n_tok || !a->n_head || a->n_head % p->n_head_kv)
 		return "n_tok is 0, or n_head no multiple of n_head_kv";
-	if ((uint64_t)a->n_seq * a->n_tok * a->n_head > (1ull << 25) || a->n_group > a->n_seq)
+	if ((uint64_t)a->n_seq * a->n_tok * a->n_head > (1ull << 25) || a->n_seq > ATTN_MAX_SEQS ||
+	    a->n_group > a->n_seq || a->n_group > ATTN_MAX_GROUPS)
 		return "the batch is larger than the call takes";
 	if (a->out_type != TYPE_F32 && a->out_type != p->type)
 		return "out_type is neither fp32 nor the cache's type";

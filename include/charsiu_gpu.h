@@ -429,7 +429,7 @@ CHARSIU_GPU_API int charsiu_gpu_pages_append_dev(struct charsiu_gpu *g,
  * for all of the group's queries. (Only pages that every query of the group sees
  * whole are taken so; the rest is read through each sequence's own table.)
  * n_group 0: group and shared may be NULL. Sequences outside all groups share
- * nothing.
+ * nothing. n_seq is at most 65536, n_group 4096, n_seq * n_tok * n_head 2^25.
  *
  * max_len: about the longest length; results hold for any, the split of the work
  * over the GPU is chosen by it. */

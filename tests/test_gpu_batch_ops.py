@@ -557,7 +557,8 @@ def test_attention_of_many_groups_and_sequences(layer):
     """More sequences than the rows kernel's estimate looks at, more groups than a warp has lanes, pads and
     empty sequences inside the groups, a scale below 0."""
     rng = np.random.default_rng(31)
-    for groups, each, t, heads, scale in ((40, 4, 1, 8, None), (3, 50, 2, 4, -0.07), (1, 140, 1, 8, -0.2)):
+    for groups, each, t, heads, scale in ((40, 4, 1, 8, None), (3, 50, 2, 4, -0.07), (1, 140, 1, 8, -0.2),
+                                           (350, 3, 1, 4, None)):
         sizes = [[int(v) for v in rng.integers(t, 60, each)] for _ in range(groups)]
         for g in sizes:
             g[1] = t                       # as short as can be
@@ -572,6 +573,16 @@ def test_attention_of_many_groups_and_sequences(layer):
         out = run_attention(layer, c, slots, bounds, shared, t, heads, q, scale=scale)
         known = [s if s < len(lens) else -1 for s in slots]
         check_attention(c, known, lens, table, t, heads, q, out, scale=scale)
+
+
+def test_attention_of_as_many_sequences_and_groups_as_a_call_takes(layer):
+    rng = np.random.default_rng(35)
+    sizes = [[1 + (i + j) % 9 for j in range(16)] for i in range(4096)]
+    c, slots, bounds, lens, table = build_batch(layer, rng, sizes, [1] * 4096, 1, 2, 1, 64, 16, BF16, layers=1, at=0)
+    q = queries(rng, 65536, 2, 64, BF16)
+    out = run_attention(layer, c, slots, bounds, [1] * 4096, 1, 2, q, at=0)
+    some = np.concatenate((np.arange(40), np.arange(30000, 65536, 777), np.arange(65500, 65536)))
+    check_attention(c, [slots[i] for i in some], lens, table, 1, 2, q[some], out[some], at=0)
 
 
 def test_attention_with_a_scale_of_0(layer):
@@ -705,10 +716,13 @@ def test_attention_refusals(layer):
     b, w = batch()
     layer.attention_dev(c.p, 0, b, q.data_ptr(), out.data_ptr(), st())
     for changes in (dict(slots=None), dict(group=None), dict(shared=None), dict(n_tok=0), dict(n_head=0), dict(n_head=3),
-                    dict(out_type=F16), dict(n_group=3), dict(work=None), dict(work_bytes=100)):
+                    dict(out_type=F16), dict(n_group=3), dict(work=None), dict(work_bytes=100), dict(n_seq=65537),
+                    dict(n_seq=8192, n_group=4097), dict(n_tok=1 << 23)):
         b, w = batch(**changes)
         with pytest.raises(GpuError):
             layer.attention_dev(c.p, 0, b, q.data_ptr(), out.data_ptr(), st())
+    for changes in (dict(n_seq=65537), dict(n_seq=8192, n_group=4097), dict(n_tok=1 << 23)):
+        assert layer.attention_work(c.p, batch(**changes)[0]) == 0
     b, w = batch()
     for args in ((2, q.data_ptr(), out.data_ptr()), (0, 0, out.data_ptr()), (0, q.data_ptr(), out.data_ptr() + 2)):
         with pytest.raises(GpuError):
