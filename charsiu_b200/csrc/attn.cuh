@@ -447,7 +447,10 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 			h.len = attn_slot_len(a, slot);
 			int32_t k0 = h.len ? shared : 0;
 			uint32_t kind = own ? (!piece && !k0 ? 32u : 0u) : 16u;  // 32: no prefix, its first piece says so
-			h.k1 = h.len;
+			// (no keys behind the tile's last query's position: 4 prompts of 1000 tokens, 32 heads of
+			// 128, 498 us, with all the sequence's keys for every tile 769)
+			const uint32_t last = (min((h.tile + 1) * ATTN_TILE_ROWS, tg) - 1) / a.gqa;
+			h.k1 = max(h.len - (int32_t)a.n_tok + (int32_t)last + 1, 0);
 			h.slot_at = (own ? a.pre_splits : 0) + piece;
 			if (own)
 				attn_piece(k0, h.k1, piece, a.own_splits, a.own_grain);
