@@ -3,8 +3,8 @@
 // (charsiu_gpu_adapters_dev): y_r = base_r + scale_a B_a (A_a x_r), a = which[r].
 //
 // The first launch makes t_r = A_a x_r (rank numbers a row): K is cut into pieces whose sums
-// go to scratch. The last adds the pieces up and makes y (in long batches a launch between
-// them adds up). Both take tiles of 16 rows, as mma.sync's m, in long batches four of them. A
+// go to scratch. The last adds the pieces up and makes y (where that is much to read a launch
+// between them adds up). Both take tiles of 16 rows, as mma.sync's m, in long batches four of them. A
 // tile's rows may want different adapters: each of its distinct ones is a product of its
 // own over all 16 rows, of which only the rows that want it are kept (so whatever an
 // adapter's weights are, they reach no other row). In a long prompt a tile has one; in a
@@ -50,6 +50,7 @@ struct AdaptArgs {
 	float *t;               // [set][piece][row][RT]
 	uint32_t n_sets, m, k;
 	uint32_t pieces;        // of K
+	uint32_t left;          // of them, for the last launch to add up: all, or 1 behind adapt_sum_kernel
 	uint32_t parts;         // the first launch: CTAs that share a tile's distinct adapters
 	uint32_t cols;          // the second: columns a CTA, a multiple of 32
 	uint32_t blocks;        // and CTAs over all sets' columns
@@ -291,7 +292,7 @@ adapt_expand_kernel(const __grid_constant__ AdaptArgs a)
 		for (uint32_t i = threadIdx.x; i < ADAPT_ROWS * RT; i += ADAPT_WARPS * 32) {
 			float v = 0.0f;
 #pragma unroll 4
-			for (uint32_t p = 0; p < a.pieces; p++)
+			for (uint32_t p = 0; p < a.left; p++)
 				v += i < filled ? t[(size_t)p * a.m * RT + i] : 0.0f;
 			s_t[i / RT][i % RT] = v;          // (rows that want no adapter: never used)
 		}
@@ -394,7 +395,7 @@ adapt_expand_kernel(const __grid_constant__ AdaptArgs a)
 // adapter's weights pass through shared memory once for all of them (a prompt's rows
 // share their adapter; where they do not, a warp without rows of an adapter sits
 // it out). 2000 rows, K = N = 4096, rank 64: 16 + 3 + 25 us, against 28 + 58 by the kernels
-// above, which read every weight again for each 16 rows. Adapters one at a time, not two:
+// above (then without a sum of their own), which read every weight again for each 16 rows. Adapters one at a time, not two:
 // 48 us for that, 145 against 113 for 1000 rows of 8 mixed adapters (but 38 against 42 for
 // 2000 rows of one).
 constexpr uint32_t ADAPT_LONG_ROWS = 64, ADAPT_STAGES = 3;

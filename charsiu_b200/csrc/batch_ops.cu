@@ -341,18 +341,18 @@ uint32_t adapters_ranks(const charsiu_gpu_adapters *s, unsigned n)
 
 constexpr uint32_t ADAPT_CTAS_PER_SM = 4, ADAPT_MAX_PIECES = 16, ADAPT_LONG_CTAS_PER_SM = 3;
 constexpr unsigned ADAPT_LONG_M = 512;
+constexpr uint32_t ADAPT_SUM_BYTES = 32768;
 
-// Whether the rows go 64 to a CTA. Measured, K = N = 4096, 16 rows a CTA against 64: of rank 16
-// 256 rows 13 against 19 us, 512 rows 18 against 18, 1000 rows 31 against 29; of rank 64 128 rows
-// 31 against 33, 256 rows 35 against 28, 512 rows 46 against 32, 1000 rows 56 against 38. With the
-// rows' adapters mixed, 256 rows of rank 16 32 against 35 us, of rank 64 68 against 56.
+// Whether the rows go 64 to a CTA. Measured, K = N = 4096, 16 rows a CTA against 64: 256 rows of rank
+// 16, 32, 64 12.6 / 18.6, 17.8 / 21.2, 25 / 28 us; 512 rows 17.5 / 18.4, 24 / 21, 37 / 32; 1000 rows
+// 31 / 29, 40 / 31, 51 / 38. With 8 adapters mixed over the rows, 256 rows 32 / 35, 43 / 42, 58 / 56;
+// 512 rows 54 / 45, 74 / 55, 102 / 90.
 bool adapters_long(const charsiu_gpu_adapters *s, unsigned n, unsigned m)
 {
 	for (unsigned i = 0; i < n; i++)
 		if (s[i].max_rank % 8)          // (weights are copied by 16 bytes)
 			return false;
-	const uint32_t ranks = adapters_ranks(s, n);
-	return ranks <= 64 && m >= (ranks == 64 ? ADAPT_LONG_M / 2 : ADAPT_LONG_M);
+	return m >= ADAPT_LONG_M && adapters_ranks(s, n) <= 64;
 }
 
 // pieces of K: enough CTAs to fill the GPU, at least one 32-block a warp
@@ -378,7 +378,7 @@ size_t adapters_bytes(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n,
 }
 
 template <typename T, int RT>
-int adapters(charsiu_gpu *g, const AdaptArgs &a, bool lng, void *stream)
+int adapters(charsiu_gpu *g, AdaptArgs &a, bool lng, void *stream)
 {
 	if constexpr (RT <= 64) {
 		if (lng) {
@@ -400,8 +400,19 @@ int adapters(charsiu_gpu *g, const AdaptArgs &a, bool lng, void *stream)
 		}
 	}
 	const unsigned tiles = (a.m + ADAPT_ROWS - 1) / ADAPT_ROWS;
+	// Every CTA of the columns adds the pieces of its rows up, or a launch before them does, where that
+	// is much to read. Measured, K = N = 4096, 16 pieces, in the CTAs against by a launch: 16
+	// rows of rank 16 (16 KB a CTA) 10.8 against 12.6 us, of rank 32 13.0 / 13.0, 64 20 / 16, 128
+	// 33 / 23; 128 rows 11.4 / 12.6, 18 / 16, 31 / 22, 89 / 48; 4 rows of rank 32 8.0 / 10.3,
+	// 128 17.4 / 17.2.
+	const bool sum = a.pieces > 1 && (a.m < ADAPT_ROWS ? a.m : ADAPT_ROWS) * RT * sizeof(float) * a.pieces >=
+						 ADAPT_SUM_BYTES;
+	const uint32_t each = a.m * (RT / 4);
+	a.left = sum ? 1 : a.pieces;
 	return launch(g, stream, adapt_shrink_kernel<T, RT>, dim3(tiles, a.pieces * a.parts, a.n_sets),
 		      ADAPT_WARPS * 32, 0, a) &&
+			       (!sum || launch(g, stream, adapt_sum_kernel, dim3((each + 255) / 256, a.n_sets), 256, 0,
+					       (float4 *)a.t, a.pieces, each)) &&
 			       launch(g, stream, adapt_expand_kernel<T, RT>, dim3(tiles, a.blocks),
 				      ADAPT_WARPS * 32, 0, a)
 		       ? 0
@@ -409,7 +420,7 @@ int adapters(charsiu_gpu *g, const AdaptArgs &a, bool lng, void *stream)
 }
 
 template <typename T>
-int adapters_of(charsiu_gpu *g, const AdaptArgs &a, uint32_t ranks, bool lng, void *stream)
+int adapters_of(charsiu_gpu *g, AdaptArgs &a, uint32_t ranks, bool lng, void *stream)
 {
 	switch (ranks) {
 	case 8: return adapters<T, 8>(g, a, lng, stream);
