@@ -299,6 +299,8 @@ adapt_expand_kernel(const __grid_constant__ AdaptArgs a)
 	}
 	__syncthreads();
 	const uint32_t end = min(col0 + a.cols, set.n), groups = (end - col0 + 7) / 8;
+	// a column of 4 ranks, beside sets whose ranks make RT, is 8 bytes of B, all of them lane 0's
+	const bool narrow = set.max_rank < 8;
 	// two columns a load and store
 	const bool pairs = set.n % 2 == 0 && !(((uintptr_t)set.base | (uintptr_t)set.y) & 7);
 	// rows of no adapter keep the base's bits
@@ -328,8 +330,11 @@ adapt_expand_kernel(const __grid_constant__ AdaptArgs a)
 				it.w[0] = ok ? *(const uint32_t *)src : 0u;
 			} else if (SP == 4) {
 				*(uint2 *)it.w = ok ? *(const uint2 *)src : make_uint2(0, 0);
-			} else {
+			} else if (!narrow) {
 				*(uint4 *)(it.w + x / 2) = ok ? *(const uint4 *)(src + x) : make_uint4(0, 0, 0, 0);
+			} else {
+				const uint2 v = ok ? *(const uint2 *)src : make_uint2(0, 0);
+				*(uint4 *)(it.w + x / 2) = make_uint4(v.x, v.y, 0, 0);
 			}
 		}
 #pragma unroll

@@ -821,6 +821,34 @@ def test_adapters(layer, m, k, ns, slots, max_rank, ty):
             check_adapters(q, d, which, mats, ranks, scale, bases, ys)
 
 
+@pytest.mark.parametrize("m,max_ranks,ty", [
+    (5, (4, 24), F16), (16, (64, 4), BF16), (21, (128, 4, 8), BF16), (33, (4, 32, 16), F16), (17, (8, 16, 4), BF16),
+    (40, (8, 128), F16), (30, (24, 128, 64), BF16), (520, (4, 64), BF16), (530, (128, 4), F16), (515, (8, 64, 16), F16),
+    (540, (64, 40), BF16)], ids=str)
+def test_adapters_of_sets_of_different_rank(layer, m, max_ranks, ty):
+    """Each set has a max_rank of its own, its columns of B as wide as that: odd N, ranks up to the whole
+    of it, B's arrays as long as they have to be."""
+    rng = np.random.default_rng(m + sum(max_ranks))
+    k, slots, ns = 160, 5, [33, 130, 7][:len(max_ranks)]
+    made = [make_adapters(rng, slots, r, k, [n], ty, ranks=[r, 1, 0, r, min(r, 3)]) for r, n in zip(max_ranks, ns)]
+    dm = [(mats[0][0].cuda(), mats[0][1].cuda(), dev(np.array(ranks, np.int32)), dev(scale)) for mats, ranks, scale in made]
+    sets = layer.adapter_sets([AdaptersStruct(a=a.data_ptr(), b=b.data_ptr(), rank=rk.data_ptr(), scale=sc.data_ptr(), k=k,
+                                              n=b.shape[1], slots=slots, max_rank=a.shape[1], type=ty) for a, b, rk, sc in dm])
+    q = rng.integers(-127, 128, (m, k)).astype(np.int8)
+    d = (0.001 + 0.02 * rng.random((m, k // 32))).astype(np.float32)
+    bases = [rng.standard_normal((m, n)).astype(np.float32) for n in ns]
+    dq, dd, db = dev(q), dev(d), [dev(b) for b in bases]
+    w = scratch(layer.adapters_work(sets, m))
+    mixed = rng.integers(-1, slots + 1, m).tolist()
+    for which in (mixed, sorted(mixed)):
+        wh, ys = dev(np.array(which, np.int32)), [torch.full_like(b, 9.0) for b in db]
+        layer.adapters_dev(sets, m, dq.data_ptr(), dd.data_ptr(), wh.data_ptr(), layer.pointers([b.data_ptr() for b in db]),
+                           layer.pointers([y.data_ptr() for y in ys]), w.data_ptr(), w.numel(), st())
+        torch.cuda.synchronize()
+        for (mats, ranks, scale), base, y in zip(made, bases, ys):
+            check_adapters(q, d, which, mats, ranks, scale, [base], [y.cpu().numpy()])
+
+
 def test_adapters_rows_keep_apart(layer):
     """inf and NaN in one request's adapter, activation or base reach no other request; rank 0 adds 0, a rank out
     of range is cut to the table's."""
