@@ -23,12 +23,12 @@
 #pragma once
 
 #include "attn.cuh"
+#include "batch_checks.h"
 #include "charsiu_gpu.h"
 #include "ptx.cuh"
 
 namespace cgpu {
 
-constexpr int ADAPT_MAX_SETS = 8;
 constexpr uint32_t ADAPT_ROWS = 16;
 constexpr uint32_t ADAPT_WARPS = 4;
 

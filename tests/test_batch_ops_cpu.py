@@ -99,3 +99,15 @@ def test_the_plain_pages_keep_their_books():
             assert p.compact() == (p.ref > 0).sum() and not p.ref[(p.ref > 0).sum():].any()
         check()
     assert p.refused > 0
+
+
+def test_the_checks_of_sizes_and_pointers(tmp_path):
+    """batch_checks.h by itself: sizes whose product passes 64 bits among them."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "batch_checks")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", f"-I{root}/include", f"-I{root}/charsiu_b200/csrc",
+                    f"{root}/tests/batch_checks_check.cpp", "-o", exe], check=True)
+    got = subprocess.run([exe], capture_output=True, text=True)
+    assert got.returncode == 0 and got.stdout.startswith("ok "), got.stdout
