@@ -16,6 +16,8 @@ inline bool misaligned(const void *p, uintptr_t to)
 	return (uintptr_t)p & (to - 1);
 }
 
+constexpr uint32_t PAGES_MAX_ITEMS = 1024;      // slots a call lists, one a thread of its planner
+
 // "" or why the calls would refuse this cache
 inline const char *pages_fault(const charsiu_gpu_pages *p)
 {
@@ -39,6 +41,18 @@ inline const char *pages_fault(const charsiu_gpu_pages *p)
 		return "a stride of the cache is not a multiple of 8";
 	if (p->pos_stride < p->head_dim || p->head_stride < p->head_dim)
 		return "the cache's positions or heads overlap";
+	return "";
+}
+
+// "" or why the calls would refuse this list of slots
+inline const char *slots_fault(const int32_t *slots, unsigned n)
+{
+	if (n && !slots)
+		return "no slots";
+	if (n > PAGES_MAX_ITEMS)
+		return "more slots than a call takes";
+	if (n && misaligned(slots, 4))
+		return "a list of slots is misaligned";
 	return "";
 }
 

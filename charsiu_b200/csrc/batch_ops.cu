@@ -113,11 +113,8 @@ int slots_check(charsiu_gpu *g, const charsiu_gpu_pages *p, const int32_t *slots
 {
 	if (pages_check(g, p, true))
 		return -1;
-	if (n && !slots)
-		return refuse(g, "no slots");
-	if (n > PAGES_MAX_ITEMS)
-		return refuse(g, "more slots than a call takes");
-	return 0;
+	const char *why = slots_fault(slots, n);
+	return *why ? refuse(g, why) : 0;
 }
 
 template <typename T>

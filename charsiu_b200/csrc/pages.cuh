@@ -13,12 +13,12 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "batch_checks.h"
 #include "charsiu_gpu.h"
 #include "ptx.cuh"
 
 namespace cgpu {
 
-constexpr uint32_t PAGES_MAX_ITEMS = 1024;      // slots a call lists, one a thread of its planner
 constexpr int PAGES_PLAN_THREADS = 1024;
 
 // The words of `work`: [0] the refused items so far; [1] the moves of a compaction.

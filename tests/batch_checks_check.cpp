@@ -83,10 +83,22 @@ void attention_sizes()
 	expect(false, attention_fault(&p, &none), "attention of nothing");
 }
 
+// a list that the planners would read misaligned (a fault there) is refused on the host
+void lists_of_slots()
+{
+	for (uintptr_t off = 0; off < 8; off++)
+		expect(off % 4 != 0, slots_fault(at<const int32_t>(4096 + off), 3), "slots at", off);
+	expect(false, slots_fault(at<const int32_t>(4098), 0), "no slots");
+	expect(true, slots_fault(nullptr, 1), "null slots");
+	expect(false, slots_fault(at<const int32_t>(4096), 1024), "1024 slots");
+	expect(true, slots_fault(at<const int32_t>(4096), 1025), "1025 slots");
+}
+
 } // namespace
 
 int main()
 {
+	lists_of_slots();
 	attention_sizes();
 	if (wrong)
 		return 1;

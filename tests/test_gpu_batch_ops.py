@@ -296,6 +296,24 @@ def test_pages_refusals(layer):
         layer.pages_free_dev(c.p, s.data_ptr(), 1, st())
 
 
+def test_pages_lists_that_are_misaligned(layer):
+    """A list of slots at an odd address is refused on the host (the planners read whole words)."""
+    c = Cache(layer, np.random.default_rng(1), n_seq=3, max_pages=4, n_pages=5)
+    s = c.ints([0, 1, 2])
+    for off in (1, 2, 3):
+        bad = s.data_ptr() + off
+        with pytest.raises(GpuError):
+            layer.pages_grow_dev(c.p, bad, 1, 1, st())
+        with pytest.raises(GpuError):
+            layer.pages_free_dev(c.p, bad, 1, st())
+        for src, dst in ((bad, s.data_ptr()), (s.data_ptr(), bad)):
+            with pytest.raises(GpuError):
+                layer.pages_fork_dev(c.p, src, dst, 1, st())
+    layer.pages_grow_dev(c.p, s.data_ptr() + 4, 2, 1, st())
+    torch.cuda.synchronize()
+    assert c.len.tolist() == [0, 1, 1]
+
+
 # ---- the append --------------------------------------------------------------------
 
 
