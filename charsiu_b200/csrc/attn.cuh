@@ -19,6 +19,7 @@
 
 #include <type_traits>
 
+#include "attn_cut.h"
 #include "charsiu_gpu.h"
 #include "pages.cuh"
 #include "ptx.cuh"
@@ -170,19 +171,6 @@ __device__ __forceinline__ bool attn_find_unit(const AttnArgs &a, uint32_t u, ui
 		before += __shfl_sync(0xffffffffu, inc, 31);
 	}
 	return false;
-}
-
-// Piece `i` of `n` of the keys [k0, k1): whole grains
-__device__ __forceinline__ void attn_piece(int32_t &k0, int32_t &k1, uint32_t i, uint32_t n,
-					   uint32_t grain)
-{
-	const int32_t keys = k1 - k0;
-	const int32_t grains = (keys + (int32_t)grain - 1) / (int32_t)grain;
-	const int32_t each = (grains + (int32_t)n - 1) / (int32_t)n * (int32_t)grain;
-	const int64_t b = (int64_t)k0 + (int64_t)i * each, e = b + each;
-	const int32_t last = k1;
-	k0 = (int32_t)(b < last ? b : last);
-	k1 = (int32_t)(e < last ? e : last);
 }
 
 // ---- mma.sync pieces ---------------------------------------------------------------

@@ -101,13 +101,23 @@ def test_the_plain_pages_keep_their_books():
     assert p.refused > 0
 
 
-def test_the_checks_of_sizes_and_pointers(tmp_path):
-    """batch_checks.h by itself: sizes whose product passes 64 bits among them."""
+def run_check(tmp_path, name):
+    """tests/<name>.cpp against the headers it includes."""
     import os
     import subprocess
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    exe = str(tmp_path / "batch_checks")
+    exe = str(tmp_path / name)
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", f"-I{root}/include", f"-I{root}/charsiu_b200/csrc",
-                    f"{root}/tests/batch_checks_check.cpp", "-o", exe], check=True)
+                    f"{root}/tests/{name}.cpp", "-o", exe], check=True)
     got = subprocess.run([exe], capture_output=True, text=True)
     assert got.returncode == 0 and got.stdout.startswith("ok "), got.stdout
+
+
+def test_the_checks_of_sizes_and_pointers(tmp_path):
+    """batch_checks.h by itself: sizes whose product passes 64 bits among them."""
+    run_check(tmp_path, "batch_checks_check")
+
+
+def test_the_cuts_of_the_longest_sequences(tmp_path):
+    """attn_cut.h by itself, up to the longest length that a cache may tell."""
+    run_check(tmp_path, "attn_cut_check")
