@@ -212,8 +212,9 @@ adapt_shrink_kernel(const __grid_constant__ AdaptArgs a)
 #pragma unroll
 			for (int x = 0; x < (int)ADAPT_WARPS; x++)
 				v += s_t[x][i / RT][i % RT];
+			// (behind the rank 0, which an infinite d times the sum's 0 is not)
 			if (rows >> (i / RT) & 1)
-				t[i] = v;
+				t[i] = i % RT < rank ? v : 0.0f;
 		}
 	}
 }
@@ -313,7 +314,9 @@ adapt_expand_kernel(const __grid_constant__ AdaptArgs a)
 		for (int j = 0; j < 4; j++) {
 			const float v = s_t[lane / 4 + 8 * (j & 1)][c * SP + 2 * ks + (j >> 1)];
 			hi[ks][j] = __float_as_uint(v) & 0xffffe000u;
-			lo[ks][j] = __float_as_uint(__fsub_rn(v, __uint_as_float(hi[ks][j])));
+			// (an infinite t is infinite in hi, and its rest is 0, not inf - inf)
+			const float top = __uint_as_float(hi[ks][j]);
+			lo[ks][j] = v == top ? 0u : __float_as_uint(__fsub_rn(v, top));
 		}
 	struct Item {
 		uint32_t w[SP / 2];
@@ -636,11 +639,18 @@ __host__ __device__ constexpr int adapt_parts()
 	return std::is_same<T, __half>::value ? 2 : 3;
 }
 
-// the power of two for a row whose largest is `top`; 1 where that is 0, inf or NaN
+template <typename T>
+__device__ __forceinline__ float adapt_largest()
+{
+	return std::is_same<T, __half>::value ? 65504.0f : __uint_as_float(0x7f7f0000u);
+}
+
+// the power of two for a row whose largest is `top`; 1 where that is 0. (Of inf, 2^-114: the row's finite
+// numbers stay finite in 16 bits.)
 __device__ __forceinline__ float adapt_lift(float top)
 {
-	const int e = (int)(__float_as_uint(top) >> 23 & 255) - 127;
-	if (!(top > 0.0f) || e == 128)
+	const int e = min((int)(__float_as_uint(top) >> 23 & 255) - 127, 127);
+	if (!(top > 0.0f))
 		return 1.0f;
 	const int x = min(max(13 - e, -126), 126);
 	return __uint_as_float((uint32_t)(x + 127) << 23);
@@ -708,7 +718,14 @@ adapt_expand_long_kernel(const __grid_constant__ AdaptArgs a)
 			for (int i = 0; i < 2 * KS; i++) {
 				uint32_t two = 0;
 				if (i < PAIRS) {
-					two = pack_pair<T>(v[2 * i], v[2 * i + 1]);
+					// (no part but the last is infinite, or the rest would be inf - inf: what is
+					// beyond T, infinities and NaN too, is left to the last)
+					float x0 = v[2 * i], x1 = v[2 * i + 1];
+					if (p < PARTS - 1) {
+						x0 = fminf(fmaxf(x0, -adapt_largest<T>()), adapt_largest<T>());
+						x1 = fminf(fmaxf(x1, -adapt_largest<T>()), adapt_largest<T>());
+					}
+					two = pack_pair<T>(x0, x1);
 					T x[2];
 					*(uint32_t *)x = two;
 					v[2 * i] = __fsub_rn(v[2 * i], to_float<T>(x[0]));

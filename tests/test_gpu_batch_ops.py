@@ -924,6 +924,71 @@ def test_adapters_of_any_size_of_activation(layer, ty, size):
                    run_adapters(layer, mats, ranks, scale, q, d, which, [base], ty=ty))
 
 
+@pytest.mark.parametrize("ty", [BF16, F16])
+@pytest.mark.parametrize("m", [20, 520])
+def test_adapters_of_infinite_t(layer, m, ty):
+    """A t that passes fp32 gives outputs of B's sign and infinite, not NaN; what a rank leaves out adds 0 to
+    an infinite activation too; a t next to fp32's largest is finite."""
+    rng = np.random.default_rng(7)
+    k, n, r = 64, 36, 16
+    a = torch.zeros(4, r, k)
+    a[:, 0, :32] = 1                       # t's first rank: the first block; the others: the second
+    a[:, 1:, 32:] = torch.from_numpy(rng.standard_normal((4, r - 1, 32)).astype(np.float32))
+    a[3, 0, 1:32] = 0                      # (adapter 3: one element of it)
+    b = torch.from_numpy((np.sign(rng.standard_normal((4, n, r))) * (0.5 + rng.random((4, n, r)))).astype(np.float32))
+    b[3] *= 2.0 ** -10
+    mats, ranks, scale = [(a.to(TYPES[ty]), b.to(TYPES[ty]))], [16, 16, 0, 16], np.ones(4, np.float32)
+    q = rng.integers(1, 128, (m, k)).astype(np.int8)
+    q[:, 0] = 127
+    d = (0.01 + 0.01 * rng.random((m, k // 32))).astype(np.float32)
+    which = [i % 5 - 1 for i in range(m)]
+    kind = [(i // 5) % 4 for i in range(m)]
+    for i in range(m):
+        if which[i] == 3:                  # finite, but more than the largest bf16 and its half step
+            d[i, 0] = [3.4e38 / 127, 3.395e38 / 127, 3.397e38 / 127, 1][kind[i]]
+        else:
+            d[i, 0] = [np.inf, 3e37, -np.inf, 0.01][kind[i]]
+    base = rng.standard_normal((m, n)).astype(np.float32)
+    y = run_adapters(layer, mats, ranks, scale, q, d, which, [base], ty=ty)[0]
+    sign = np.sign(b.numpy()[:, :, 0])
+    plain = [i for i in range(m) if which[i] in (0, 1) and kind[i] == 3 or which[i] in (-1, 3)]
+    check_adapters(q[plain], d[plain], [which[i] for i in plain], mats, ranks, scale, [base[plain]], [y[plain]])
+    for i in range(m):
+        if which[i] == 2:
+            assert np.array_equal(y[i], base[i])
+        elif which[i] in (0, 1) and kind[i] == 1:
+            assert np.array_equal(y[i], sign[which[i]] * np.float32(np.inf)), i
+        elif which[i] in (0, 1) and kind[i] != 3:
+            assert np.isnan(y[i]).all(), i     # (inf times A's zeros in the other ranks)
+
+
+@pytest.mark.parametrize("ty", [BF16, F16])
+@pytest.mark.parametrize("m", [20, 520])
+def test_adapters_of_infinite_activations(layer, m, ty):
+    """An infinite d: every t is infinite, so y is where B's row has one sign, and NaN where it has both."""
+    rng = np.random.default_rng(8)
+    k, n, r = 96, 40, 24
+    a = torch.from_numpy((0.1 + rng.random((2, r, k))).astype(np.float32))
+    sign = rng.choice([-1, 1], (2, n)).astype(np.float32)
+    b = (0.1 + rng.random((2, n, r))).astype(np.float32) * sign[:, :, None]
+    b[:, ::7, 5] *= -1
+    mats, ranks, scale = [(a.to(TYPES[ty]), torch.from_numpy(b).to(TYPES[ty]))], [24, 19], np.ones(2, np.float32)
+    q = rng.integers(1, 128, (m, k)).astype(np.int8)
+    d = (0.01 + 0.01 * rng.random((m, k // 32))).astype(np.float32)
+    hot = rng.random(m) < 0.5
+    d[hot, 1] = np.where(rng.random(m) < 0.5, np.inf, -np.inf)[hot]
+    which = (np.arange(m) % 3 - 1).tolist()
+    base = rng.standard_normal((m, n)).astype(np.float32)
+    y = run_adapters(layer, mats, ranks, scale, q, d, which, [base], ty=ty)[0]
+    cold = [i for i in range(m) if not hot[i] or which[i] < 0]
+    check_adapters(q[cold], d[cold], [which[i] for i in cold], mats, ranks, scale, [base[cold]], [y[cold]])
+    for i in range(m):
+        if hot[i] and which[i] >= 0:
+            want = sign[which[i]] * d[i, 1]
+            want[::7] = np.nan
+            assert np.array_equal(y[i], want, equal_nan=True), i
+
+
 def test_adapters_refusals(layer):
     rng = np.random.default_rng(6)
     mats, ranks, scale = make_adapters(rng, 2, 8, 64, [10], BF16)
