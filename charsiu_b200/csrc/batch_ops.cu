@@ -277,12 +277,56 @@ bool adapters_long(const charsiu_gpu_adapters *s, unsigned n, unsigned m)
 	return m >= ADAPT_LONG_M && adapters_ranks(s, n) <= 64;
 }
 
+uint64_t adapters_tiles(bool lng, unsigned m)
+{
+	const uint64_t rows = lng ? ADAPT_LONG_ROWS : ADAPT_ROWS;
+	return (m + rows - 1) / rows;
+}
+
+// CTAs that fill the GPU
+uint64_t adapters_aim(charsiu_gpu *g, bool lng)
+{
+	return (uint64_t)(lng ? ADAPT_LONG_CTAS_PER_SM : ADAPT_CTAS_PER_SM) * layer_sms(g);
+}
+
+// columns a CTA of the last launch: as wide as still fills the GPU
+uint32_t adapters_cols(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n, unsigned m)
+{
+	const bool lng = adapters_long(s, n, m);
+	const uint64_t tiles = adapters_tiles(lng, m), aim = adapters_aim(g, lng);
+	uint64_t columns = 0;
+	for (unsigned i = 0; i < n; i++)
+		columns += s[i].n;
+	if (lng) {
+		// (as many as are on it at once: twice as many, of half the columns, take 2000 rows of
+		// rank 64 from 45 to 48 us, 1000 of mixed adapters from 113 to 128)
+		const uint64_t cols = (tiles * columns / aim + 63) / 64 * 64;
+		return cols < 64 ? 64 : cols > 1024 ? 1024 : (uint32_t)cols;
+	}
+	uint32_t cols = 256;
+	while (cols > 32 && tiles * columns / cols < aim)
+		cols /= 2;
+	return cols;
+}
+
+// "" or why a call of m rows would be refused for its size
+const char *adapters_size_fault(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n, unsigned m)
+{
+	if (m > (1u << 24))
+		return "adapters: more rows than a call takes";
+	const uint32_t cols = adapters_cols(g, s, n, m);
+	uint64_t blocks = 0;
+	for (unsigned i = 0; i < n; i++)
+		blocks += ((uint64_t)s[i].n + cols - 1) / cols;
+	return blocks > 65535 ? "adapters: more columns than a call takes" : "";
+}
+
 // pieces of K: enough CTAs to fill the GPU, at least one 32-block a warp
 uint32_t adapters_pieces(charsiu_gpu *g, const charsiu_gpu_adapters *s, unsigned n, unsigned m)
 {
 	const bool lng = adapters_long(s, n, m);
-	const uint64_t rows = lng ? ADAPT_LONG_ROWS : ADAPT_ROWS, tiles = n * ((m + rows - 1) / rows);
-	uint64_t want = (uint64_t)(lng ? ADAPT_LONG_CTAS_PER_SM : ADAPT_CTAS_PER_SM) * layer_sms(g) / (tiles ? tiles : 1);
+	const uint64_t tiles = n * adapters_tiles(lng, m);
+	uint64_t want = adapters_aim(g, lng) / (tiles ? tiles : 1);
 	const uint32_t most = (s->k / 32 + ADAPT_WARPS - 1) / ADAPT_WARPS;
 	want = want < most ? want : most;
 	want = want < ADAPT_MAX_PIECES ? want : ADAPT_MAX_PIECES;
@@ -547,7 +591,7 @@ int charsiu_gpu_attention_dev(struct charsiu_gpu *g, const struct charsiu_gpu_pa
 size_t charsiu_gpu_adapters_work(struct charsiu_gpu *g, const struct charsiu_gpu_adapters *sets,
 				 unsigned n, unsigned m)
 {
-	return !g || *adapters_fault(sets, n) ? 0 : adapters_bytes(g, sets, n, m);
+	return !g || *adapters_fault(sets, n) || *adapters_size_fault(g, sets, n, m) ? 0 : adapters_bytes(g, sets, n, m);
 }
 
 int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_adapters *sets,
@@ -564,12 +608,11 @@ int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_ada
 		return 0;
 	if (!q || !d || !which || !ys || misaligned(q, 16) || misaligned(d, 4) || misaligned(which, 4))
 		return refuse(g, "adapters: an array is missing or misaligned");
-	if (m > (1u << 24))
-		return refuse(g, "adapters: more rows than a call takes");
+	if (*(why = adapters_size_fault(g, sets, n, m)))
+		return refuse(g, why);
 	if (!work || misaligned(work, 16) || work_bytes < adapters_bytes(g, sets, n, m))
 		return refuse(g, "adapters: the work array is missing, misaligned or too small");
 	AdaptArgs a = {};
-	uint64_t columns = 0;
 	uint32_t slots = 0;
 	for (unsigned i = 0; i < n; i++) {
 		AdaptSet &s = a.s[i];
@@ -587,30 +630,16 @@ int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_ada
 		s.n = sets[i].n;
 		s.slots = sets[i].slots;
 		s.max_rank = sets[i].max_rank;
-		columns += s.n;
 		slots = slots > s.slots ? slots : s.slots;
 	}
-	// CTAs over the columns: as wide as still fills the GPU
 	const bool lng = adapters_long(sets, n, m);
-	const uint64_t tile = lng ? ADAPT_LONG_ROWS : ADAPT_ROWS, tiles = (m + tile - 1) / tile;
-	const uint64_t aim = (uint64_t)(lng ? ADAPT_LONG_CTAS_PER_SM : ADAPT_CTAS_PER_SM) * layer_sms(g);
-	if (lng) {
-		// (as many as are on it at once: twice as many, of half the columns, take 2000 rows of
-		// rank 64 from 45 to 48 us, 1000 of mixed adapters from 113 to 128)
-		a.cols = (uint32_t)((tiles * columns / aim + 63) / 64 * 64);
-		a.cols = a.cols < 64 ? 64 : a.cols > 1024 ? 1024 : a.cols;
-	} else {
-		a.cols = 256;
-		while (a.cols > 32 && tiles * columns / a.cols < aim)
-			a.cols /= 2;
-	}
-	uint64_t blocks = 0;
+	const uint64_t tiles = adapters_tiles(lng, m), aim = adapters_aim(g, lng);
+	a.cols = adapters_cols(g, sets, n, m);
+	uint32_t blocks = 0;
 	for (unsigned i = 0; i < n; i++) {
 		blocks += (a.s[i].n + a.cols - 1) / a.cols;
-		a.s[i].block_end = (uint32_t)blocks;
+		a.s[i].block_end = blocks;
 	}
-	if (blocks > 65535)
-		return refuse(g, "adapters: more columns than a call takes");
 	a.q = q;
 	a.d = d;
 	a.which = which;
@@ -625,7 +654,7 @@ int charsiu_gpu_adapters_dev(struct charsiu_gpu *g, const struct charsiu_gpu_ada
 	parts = parts < slots ? parts : slots;
 	parts = parts < m ? parts : m;
 	a.parts = parts < 1 ? 1 : (uint32_t)parts;
-	a.blocks = (uint32_t)blocks;
+	a.blocks = blocks;
 	OnDevice on(g);
 	const uint32_t ranks = adapters_ranks(sets, n);
 	return sets[0].type == TYPE_F16 ? adapters_of<__half>(g, a, ranks, lng, stream)

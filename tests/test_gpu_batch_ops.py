@@ -1037,6 +1037,26 @@ def test_adapters_refusals(layer):
     torch.cuda.synchronize()
 
 
+def test_adapters_scratch_of_refused_sizes_is_0(layer):
+    """The size of the scratch says what the call would: more rows or columns than it takes are 0 there too."""
+    rng = np.random.default_rng(6)
+    mats, ranks, scale = make_adapters(rng, 2, 8, 64, [10], BF16)
+    a, b = mats[0][0].cuda(), mats[0][1].cuda()
+    rk, sc, some = dev(np.array(ranks, np.int32)), dev(scale), torch.zeros(64, device="cuda")
+
+    def sets(n, max_rank=8):
+        return layer.adapter_sets([AdaptersStruct(a=a.data_ptr(), b=b.data_ptr(), rank=rk.data_ptr(), scale=sc.data_ptr(),
+                                                  k=64, n=n, slots=2, max_rank=max_rank, type=BF16)])
+    assert layer.adapters_work(sets(10), 1 << 24) > 0 and layer.adapters_work(sets(10), (1 << 24) + 1) == 0
+    wide = 256 * 65535
+    for n, m in ((wide, 16), (wide, 400), (4 * wide, 600)):      # (600 rows: 64 a CTA, up to 1024 columns)
+        assert layer.adapters_work(sets(n), m) > 0
+        assert layer.adapters_work(sets(n + 1), m) == 0
+        with pytest.raises(GpuError):
+            layer.adapters_dev(sets(n + 1), m, some.data_ptr(), some.data_ptr(), some.data_ptr(), None,
+                               layer.pointers([some.data_ptr()]), some.data_ptr(), 1 << 62, st())
+
+
 # ---- all together --------------------------------------------------------------------------
 
 
