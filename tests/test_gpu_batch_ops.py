@@ -624,6 +624,51 @@ def test_attention_of_a_whole_prompt(layer):
         check_attention(c, slots, lens, table, n_tok, 4, q, out)
 
 
+@pytest.mark.parametrize("n_tok,sizes,shared,heads,kv,hd,page,ty", [
+    (300, [[300, 420]], [0], 8, 2, 128, 16, BF16),
+    (257, [[257]], [0], 4, 4, 128, 64, F16),
+    (200, [[200, 260], [333]], [5, 0], 6, 2, 128, 32, BF16),
+    (513, [[600]], [0], 4, 1, 64, 128, BF16)])
+def test_attention_of_longer_prompts(layer, n_tok, sizes, shared, heads, kv, hd, page, ty):
+    """Hundreds of queries a sequence, whole prompts and ones that go on, in both types and head sizes."""
+    rng = np.random.default_rng(n_tok)
+    c, slots, bounds, lens, table = build_batch(layer, rng, sizes, shared, n_tok, heads, kv, hd, page, ty)
+    q = queries(rng, len(slots) * n_tok, heads, hd, ty)
+    out = run_attention(layer, c, slots, bounds, shared, n_tok, heads, q)
+    check_attention(c, slots, lens, table, n_tok, heads, q, out)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("hd,ty,t", [(128, BF16, 3), (128, F16, 40), (64, F16, 5)])
+def test_attention_takes_nothing_from_later_queries(layer, value, hd, ty, t):
+    """inf and NaN in the last position of a sequence, which only its last query sees: the others' bits stay those
+    that they have with another finite V there."""
+    rng = np.random.default_rng(24)
+    c, slots, bounds, lens, table = build_batch(layer, rng, [[t, t + 9, t + 64]], [2], t, 8, 2, hd, 16, ty)
+    q = queries(rng, 3 * t, 8, hd, ty)
+    clean = run_attention(layer, c, slots, bounds, [2], t, 8, q).view(3, t, 8, hd)
+    check_attention(c, slots, lens, table, t, 8, q, clean)
+    for s in slots:
+        c.v[1, table[s, (lens[s] - 1) // 16], (lens[s] - 1) % 16] = value
+    got = run_attention(layer, c, slots, bounds, [2], t, 8, q).view(3, t, 8, hd)
+    off = (got[:, :t - 1].float() - clean[:, :t - 1].float()).abs().max()
+    assert off <= 2 * EPS[ty] * clean.float().abs().max()
+    assert not torch.isfinite(got[:, t - 1]).any()
+
+
+def test_attention_of_sequences_outside_the_groups(layer):
+    """Groups that leave out the first and the last sequences and some between them, and a slot that is listed twice."""
+    rng = np.random.default_rng(36)
+    for hd, ty in ((64, F16), (128, BF16)):
+        c, slots, _, lens, table = build_batch(layer, rng, [[30, 4], [9, 8, 7, 6], [77, 1], [5, 40, 3]], [0, 6, 3, 4], 2, 16, 2, hd, 16, ty)
+        slots = slots + [slots[3], slots[0]]
+        q = queries(rng, len(slots) * 2, 16, hd, ty)
+        # group bounds are one list: what lies between two groups is a group that shares nothing
+        for bounds, told in (([2, 6, 8, 11], [6, 0, 4]), ([3, 6], [6]), ([8, 11], [4])):
+            out = run_attention(layer, c, slots, bounds, told, 2, 16, q)
+            check_attention(c, slots, lens, table, 2, 16, q, out)
+
+
 def test_attention_goes_by_the_lengths_of_the_replay(layer):
     """One captured call, replayed as the sequences, their groups and their shared pages change."""
     rng = np.random.default_rng(33)
@@ -865,6 +910,23 @@ def test_adapters_of_sets_of_different_rank(layer, m, max_ranks, ty):
         torch.cuda.synchronize()
         for (mats, ranks, scale), base, y in zip(made, bases, ys):
             check_adapters(q, d, which, mats, ranks, scale, [base], [y.cpu().numpy()])
+
+
+@pytest.mark.parametrize("m,k,ns,slots,max_rank,ty", [
+    (128, 4096, [72], 4, 128, BF16), (128, 4096, [40], 3, 128, F16), (16, 4096, [40, 33], 6, 64, F16), (4, 4096, [50], 3, 128, BF16),
+    (3, 4096, [50], 3, 128, F16), (600, 256, [130], 3, 128, F16)])
+def test_adapters_whose_pieces_are_added_up_first(layer, m, k, ns, slots, max_rank, ty):
+    """Short batches with many pieces of K and ranks enough that a launch of its own adds them up (and one on
+    either side of that)."""
+    rng = np.random.default_rng(m + max_rank)
+    mats, ranks, scale = make_adapters(rng, slots, max_rank, k, ns, ty, ranks=[max_rank - i for i in range(slots)])
+    q = rng.integers(-127, 128, (m, k)).astype(np.int8)
+    d = (0.001 + 0.02 * rng.random((m, k // 32))).astype(np.float32)
+    bases = [rng.standard_normal((m, n)).astype(np.float32) for n in ns]
+    mixed = rng.integers(-1, slots + 1, m).tolist()
+    for which in (mixed, [slots - 1] * m):
+        ys = run_adapters(layer, mats, ranks, scale, q, d, which, bases, False, ty)
+        check_adapters(q, d, which, mats, ranks, scale, bases, ys)
 
 
 def test_adapters_rows_keep_apart(layer):
