@@ -19,7 +19,8 @@
 // Precision: x is q d with q int8, exact in both 16-bit types, so a 32-block's products
 // with A are exact and its sum is taken in fp32 before d scales it. t stays fp32: for its
 // product with B it is cut into parts of which each product with B is exact, two of tf32
-// (what is lost is 2^-22 of a term), in long batches two or three of B's type (see there).
+// (what is lost is less than 2^-21 of a term: the last two bits of fp32's 24), in long
+// batches two or three of B's type (see there).
 #pragma once
 
 #include "attn.cuh"

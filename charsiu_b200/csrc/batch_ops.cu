@@ -159,7 +159,9 @@ bool attention_plan(charsiu_gpu *g, const charsiu_gpu_pages *p, const charsiu_gp
 	a->pre_units = a->pre_splits = a->rows_splits = 0;
 	if (!b->n_group)
 		return false;
-	// The tensor cores' form from 32 rows of a KV head on. Measured with 4 rows a sequence, hd 64, against
+	// The tensor cores' form from 32 rows of a KV head on, over all groups; measured with one group. (Of
+	// many small groups each fills a unit of its own, and the splits below, made from the rows of all, come
+	// out as for one.) Measured with 4 rows a sequence, hd 64, against
 	// 16 rows at a time in the rows kernel: 256 shared keys, 2 sequences 9.2 against 8.6 us, 16
 	// 10.0 / 13.5; 4096, 8 20.7 / 17.4, 32 23.6 / 24.1, 64 27 / 37; 16384, 8 30.9 / 26.7, 16
 	// 32 / 35, 64 40 / 100. Of hd 128, 256, 8 11.5 / 13.1; 16384, 4 36 / 31, 8 37 / 40, 64 49 / 176.

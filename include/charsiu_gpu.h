@@ -324,7 +324,10 @@ CHARSIU_GPU_API unsigned charsiu_gpu_decoder_launches(const struct charsiu_gpu_d
  * scratch included, is the caller's: calls that may run at the same time (two
  * streams, two captured graphs) need scratch of their own. Arrays that say where
  * to read or write (slots, tables, adapter numbers) are device memory and are
- * checked there: an index out of range reads and writes nothing.
+ * checked there: an index out of range reads and writes nothing. A wait inside a
+ * kernel that gave up (after a second; none does in a sound run) leaves wrong
+ * results and shows in charsiu_gpu_kernel_error only, which a caller asks once a
+ * step or so, after synchronising.
  * No counterpart in the reference, which decodes one token at a time.
  */
 
@@ -353,9 +356,9 @@ CHARSIU_GPU_API int charsiu_gpu_norm_quantise_dev(struct charsiu_gpu *g, const f
  *
  * A call that lists slots takes them in order; one that cannot be done (a slot out
  * of range or listed before, no room in the table, no free page) is left as it was
- * and counted in the first int32 of `work`, which only the caller clears. Fresh
- * pages are the free ones of the lowest numbers, so results never depend on
- * timing. */
+ * and counted in the first int32 of `work`, which only the caller clears. Lists of
+ * slots are 4-byte aligned. Fresh pages are the free ones of the lowest numbers, so
+ * results never depend on timing. */
 struct charsiu_gpu_pages {
 	void *k, *v;                       /* 16-byte aligned */
 	int32_t *table;                    /* [n_seq][max_pages] */
@@ -419,9 +422,10 @@ CHARSIU_GPU_API int charsiu_gpu_pages_append_dev(struct charsiu_gpu *g,
  * before it. Query head h reads KV head h / (n_head / n_head_kv).
  *   out = softmax(scale * q K^T) V
  * with fp32 scores, maxima, sums and accumulators; the weights are rounded to the
- * cache's type for their product with V, the result once to out_type. A query that
- * sees nothing (position below 0, an empty or padded slot) gives zeros. What lies
- * behind a query's position never reaches its result, NaN and inf included.
+ * cache's type for their product with V (whatever out_type is), the result once to
+ * out_type. A query that sees nothing (position below 0, an empty or padded slot)
+ * gives zeros, and so does one all of whose scores are -inf. What lies behind a
+ * query's position never reaches its result, NaN and inf included.
  *
  * Sequences that share their first pages: group g is sequences group[g] to
  * group[g + 1] - 1 (ascending, device), whose slots hold the same first shared[g]
@@ -429,7 +433,8 @@ CHARSIU_GPU_API int charsiu_gpu_pages_append_dev(struct charsiu_gpu *g,
  * for all of the group's queries. (Only pages that every query of the group sees
  * whole are taken so; the rest is read through each sequence's own table.)
  * n_group 0: group and shared may be NULL. Sequences outside all groups share
- * nothing. n_seq is at most 65536, n_group 4096, n_seq * n_tok * n_head 2^25.
+ * nothing. n_seq is at most 65536, n_group 4096 and no more than n_seq, n_seq *
+ * n_tok * n_head 2^25.
  *
  * max_len: about the longest length; results hold for any, the split of the work
  * over the GPU is chosen by it. */
@@ -475,12 +480,16 @@ CHARSIU_GPU_API size_t charsiu_gpu_adapters_work(struct charsiu_gpu *g,
 						 unsigned m);
 /* ys[i][r] = bases[i][r] + scale * B (A x_r) of adapter which[r] of sets[i], for the
  * m rows of the q8_0 activation x = q d that the projections read (q int8 [m][K],
- * d fp32 [m][K/32]), against n <= 8 sets of the same K. bases and ys: n device
- * pointers to fp32 [m][N]; bases[i] may be ys[i], and bases NULL means ys: the
- * projections' outputs get the adapters added. No set's output may overlap
- * another's output or base. A row whose `which` is no adapter
- * (-1) is its base. fp32 products and sums throughout. work: 16-byte aligned, as
- * q is (d 4). */
+ * d fp32 [m][K/32]), against n <= 8 sets of the same K (each with slots and a
+ * max_rank of its own; m at most 2^24, the sets' N about 2^24 in all). bases and
+ * ys: n device pointers to fp32 [m][N]; bases[i] may be ys[i], and bases NULL means
+ * ys: the projections' outputs get the adapters added. No set's output may overlap
+ * another's output or base. A row whose `which` is no adapter (-1) is its base.
+ * Products are exact, sums and A x fp32. Before its product with B, A x loses less
+ * than 2^-21 of a component below 512 rows and where a max_rank is 4 or above 64;
+ * else 2^-27 in bf16, and in fp16 what is below 2^-24 of a component or 2^-38 of its
+ * row's largest (a component smaller than that adds nothing).
+ * work: 16-byte aligned, as q is (d 4). */
 CHARSIU_GPU_API int charsiu_gpu_adapters_dev(struct charsiu_gpu *g,
 					     const struct charsiu_gpu_adapters *sets, unsigned n,
 					     unsigned m, const int8_t *q, const float *d,
